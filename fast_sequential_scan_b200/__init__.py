@@ -10,5 +10,9 @@ from .scan_cuda import scan_single as scan_cu_single  # noqa: E402
 from .scan_cuda import scan_gated, set_backward_mode  # noqa: E402
 from .sequential_scan_cuda import set_deterministic  # noqa: E402
 from .workspace import check_status  # noqa: E402
+from .attention_cuda import linear_attention, linear_attention_step  # noqa: E402
+from .norm_cuda import rms_norm, rms_norm_quantized  # noqa: E402
+from .rotary_cuda import rotary, rotary_turns  # noqa: E402
 
-__all__ = ["scan_cu", "scan_cu_single", "scan_gated", "set_backward_mode", "set_deterministic", "check_status"]
+__all__ = ["scan_cu", "scan_cu_single", "scan_gated", "set_backward_mode", "set_deterministic", "check_status",
+           "linear_attention", "linear_attention_step", "rotary", "rotary_turns", "rms_norm", "rms_norm_quantized"]

@@ -57,6 +57,29 @@ class CarrySource(Structure):
                 ("push_state", c_void_p), ("push_prod", c_void_p), ("push_prod_out", c_void_p)]
 
 
+class Heads(Structure):
+    _fields_ = [("ptr", c_void_p), ("stride_b", c_int64), ("stride_t", c_int64), ("stride_h", c_int64), ("heads", c_int64), ("dim", c_int64)]
+
+
+class LinearAttention(Structure):
+    _fields_ = [("struct_bytes", c_uint32), ("dtype", c_int32), ("B", c_int64), ("T", c_int64), ("H", c_int64), ("q", Heads), ("k", Heads),
+                ("v", Heads), ("log_decay", c_void_p), ("decay_stride_b", c_int64), ("decay_stride_t", c_int64), ("decay_stride_h", c_int64),
+                ("lengths", c_void_p), ("h0", c_void_p), ("scale", c_float)]
+
+
+class NormWeight(Structure):
+    _fields_ = [("ptr", c_void_p), ("dtype", c_int32)]
+
+
+class NormOutput(Structure):
+    _fields_ = [("y", View), ("held", c_void_p), ("scales", c_void_p), ("rstd", c_void_p), ("group", c_int32)]
+
+
+class Rotary(Structure):
+    _fields_ = [("struct_bytes", c_uint32), ("interleaved", c_int32), ("inverse", c_int32), ("magnitude", c_float), ("rotary_dim", c_int64),
+                ("positions", c_void_p), ("position_stride_b", c_int64), ("position_stride_t", c_int64), ("turns", c_void_p)]
+
+
 _P = POINTER
 
 # name -> (restype, argtypes); every symbol include/fss_b200.h declares
@@ -100,6 +123,17 @@ SIGNATURES = {
                                               _P(CarrySource), c_void_p, c_void_p, c_int64]),
     "fss_seqpar_fixup_backward_from": (c_int, [_P(ScanCtx), c_int, c_int64, c_int64, c_int64] + [_P(View)] * 5
                                        + [_P(CarrySource), c_void_p, c_void_p, c_void_p, c_int64]),
+    "fss_linear_attention_workspace_bytes": (c_size_t, [_P(LinearAttention), c_int]),
+    "fss_linear_attention_forward": (c_int, [_P(ScanCtx), _P(LinearAttention), _P(Heads), c_void_p]),
+    "fss_linear_attention_backward": (c_int, [_P(ScanCtx), _P(LinearAttention), _P(Heads), c_void_p, c_void_p, _P(Heads), _P(Heads), _P(Heads),
+                                              c_void_p, c_int, c_void_p]),
+    "fss_linear_attention_step": (c_int, [_P(ScanCtx), _P(LinearAttention), _P(Heads), c_void_p, c_int64, c_int64, c_void_p]),
+    "fss_rms_norm_forward": (c_int, [_P(ScanCtx), c_int, c_int64, c_int64, c_int64, _P(View), _P(View), _P(NormWeight), c_float, _P(View),
+                                     _P(NormOutput)]),
+    "fss_rms_norm_workspace_bytes": (c_size_t, [c_int64]),
+    "fss_rms_norm_backward": (c_int, [_P(ScanCtx), c_int, c_int64, c_int64, c_int64, _P(View), _P(NormWeight), c_void_p, _P(View), _P(View),
+                                      _P(View), c_void_p]),
+    "fss_rotary_apply": (c_int, [_P(ScanCtx), c_int, c_int64, c_int64, _P(Heads), _P(Heads), c_void_p, c_void_p, _P(Rotary)]),
     "fss_scan_forward_noalloc": (c_int, [c_int, c_int, c_void_p, c_int64, c_int64, c_int64, _P(View), _P(View), _P(View)]),
 }
 

@@ -1,0 +1,230 @@
+"""Linear attention with a decay for each head: the scan of this package with a matrix for a state.
+
+For every sequence and head, with a state ``S`` of ``[key_dim, value_dim]`` in fp32,
+
+    S_t = exp(log_decay_t) * S_{t-1} + k_t v_t^T ;      o_t = scale * q_t^T S_t ,      S_{-1} = h0 (or zeros)
+
+:func:`linear_attention` takes whole sequences (training, prompts, chunks of a prompt) and is differentiable with
+respect to everything but ``lengths``; :func:`linear_attention_step` takes one token for each sequence and updates the
+states in place (decoding).
+
+Layouts: ``q`` ``[batch, seq, query_heads, key_dim]``, ``k`` ``[batch, seq, key_heads, key_dim]``, ``v`` ``[batch, seq,
+value_heads, value_dim]``, bf16 or fp32, any strides with neighbouring channels (slices of one projection's output are
+taken as they are).  The layer has as many states a sequence as the largest of the three head counts; the others divide
+it, and neighbouring heads share.  ``log_decay`` is fp32: ``[heads]`` for a constant of each head, or ``[batch, seq,
+heads]``.  A log decay of ``-inf`` empties the state before its token, which is how several documents share a row.
+
+``lengths`` ``[batch]`` (int32, on the device): the tokens of each sequence that count.  Rows behind them are not read
+(they may hold anything, NaN included); their outputs and gradients are zeros, and the last state is the one behind the
+last token that counts -- ``h0`` for an empty sequence.
+
+Sums and states are fp32; outputs and gradients are rounded once to the tensors' type.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional
+
+import torch
+from torch.autograd import Function
+from torch.autograd.function import once_differentiable
+
+from . import _lib, workspace
+
+_DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float32: _lib.DTYPE_F32}
+MAX_DIM = 256      # of keys and of values
+
+
+def _check(name: str, t: torch.Tensor, dim: int, like: Optional[torch.Tensor], dtype=None) -> None:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} must be a CUDA tensor (this library has no CPU path)")
+    if like is not None and t.device != like.device:
+        raise RuntimeError(f"{name}: on {t.device}, expected {like.device}")
+    if dtype is not None and t.dtype != dtype:
+        raise RuntimeError(f"{name}: expected dtype {dtype}, got {t.dtype}")
+    if t.dim() != dim:
+        raise RuntimeError(f"{name}: expected {dim} dimensions, got {tuple(t.shape)}")
+
+
+def _check_heads(q, k, v, log_decay, seq: bool):
+    """Validates what both entry points share; returns ``(heads, key_dim, value_dim)``."""
+    dim = 4 if seq else 3
+    what = "[batch, seq, heads, dim]" if seq else "[batch, heads, dim]"
+    _check("q", q, dim, None)
+    if q.dtype not in _DTYPES:
+        raise RuntimeError(f"q: unsupported dtype {q.dtype} (bf16 or fp32)")
+    _check("k", k, dim, q, q.dtype)
+    _check("v", v, dim, q, q.dtype)
+    if k.shape[:-2] != q.shape[:-2] or v.shape[:-2] != q.shape[:-2] or k.shape[-1] != q.shape[-1]:
+        raise RuntimeError(f"q, k, v: shapes {tuple(q.shape)}, {tuple(k.shape)} and {tuple(v.shape)} do not go together (expected {what})")
+    counts = (q.shape[-2], k.shape[-2], v.shape[-2])
+    heads = max(counts)
+    if min(counts) < 1 or any(heads % c for c in counts):
+        raise RuntimeError(f"q, k, v: {counts} heads; the largest count has to be a multiple of the others")
+    if not (1 <= q.shape[-1] <= MAX_DIM and 1 <= v.shape[-1] <= MAX_DIM):
+        raise RuntimeError(f"head dimensions {q.shape[-1]} and {v.shape[-1]}: 1 to {MAX_DIM} are supported")
+    _check("log_decay", log_decay, log_decay.dim() if isinstance(log_decay, torch.Tensor) else 1, q, torch.float32)
+    full = (*q.shape[:-2], heads)
+    if log_decay.shape != (heads,) and log_decay.shape != full:
+        raise RuntimeError(f"log_decay: expected [{heads}] or {list(full)}, got {list(log_decay.shape)}")
+    return heads, q.shape[-1], v.shape[-1]
+
+
+def _channels(t: torch.Tensor) -> torch.Tensor:
+    """A tensor the kernels can address: neighbouring channels."""
+    return t if t.shape[-1] == 1 or t.stride(-1) == 1 or t.numel() == 0 else t.contiguous()
+
+
+def _heads(t: torch.Tensor) -> _lib.Heads:
+    if t.dim() == 3:      # a token of each sequence
+        return _lib.Heads(t.data_ptr(), t.stride(0), 0, t.stride(1), t.shape[1], t.shape[2])
+    return _lib.Heads(t.data_ptr(), t.stride(0), t.stride(1), t.stride(2), t.shape[2], t.shape[3])
+
+
+def _problem(q, k, v, log_decay, lengths, h0, scale: float, heads: int, seq: int) -> _lib.LinearAttention:
+    sb, st, sh = (0, 0, log_decay.stride(0)) if log_decay.dim() == 1 else \
+        (log_decay.stride(0), 0, log_decay.stride(1)) if log_decay.dim() == 2 else log_decay.stride()
+    return _lib.LinearAttention(ctypes.sizeof(_lib.LinearAttention), _DTYPES[q.dtype], q.shape[0], seq, heads, _heads(q), _heads(k), _heads(v),
+                                log_decay.data_ptr(), sb, st, sh, lengths.data_ptr() if lengths is not None else None,
+                                h0.data_ptr() if h0 is not None else None, scale)
+
+
+def _scratch(problem: _lib.LinearAttention, backward: int, device: torch.device) -> Optional[torch.Tensor]:
+    need = _lib.lib().fss_linear_attention_workspace_bytes(ctypes.byref(problem), backward)
+    return torch.empty(need, dtype=torch.uint8, device=device) if need else None
+
+
+def _pointer(t: Optional[torch.Tensor]) -> Optional[int]:
+    return t.data_ptr() if t is not None else None
+
+
+def linear_attention_forward(q, k, v, log_decay, *, scale: float, h0=None, lengths=None, want_final: bool = False):
+    """``(o, h_last or None)`` of tensors that were checked; ``h0`` contiguous fp32."""
+    heads = max(q.shape[2], k.shape[2], v.shape[2])
+    B, T, K, V = q.shape[0], q.shape[1], q.shape[3], v.shape[3]
+    q, k, v = _channels(q), _channels(k), _channels(v)
+    o = torch.empty(B, T, heads, V, dtype=v.dtype, device=v.device)
+    h_last = torch.empty(B, heads, K, V, dtype=torch.float32, device=v.device) if want_final else None
+    p = _problem(q, k, v, log_decay, lengths, h0, scale, heads, T)
+    scratch = _scratch(p, 0, v.device)
+    ctx, out = workspace.call_context(v.device, scratch), _heads(o)
+    _lib.check(_lib.lib().fss_linear_attention_forward(ctypes.byref(ctx), ctypes.byref(p), ctypes.byref(out), _pointer(h_last)),
+               "fss_linear_attention_forward")
+    return o, h_last
+
+
+def linear_attention_backward(q, k, v, log_decay, grad_o, *, scale: float, h0=None, lengths=None, h_last=None, grad_last=None,
+                              want=(True, True, True, False, False)):
+    """``[dq, dk, dv, dlog_decay, dh0]``, None for those that ``want`` does not ask for."""
+    heads = max(q.shape[2], k.shape[2], v.shape[2])
+    B, T, K, V = q.shape[0], q.shape[1], q.shape[3], v.shape[3]
+    q, k, v, grad_o = _channels(q), _channels(k), _channels(v), _channels(grad_o)
+    new = lambda t: torch.empty(t.shape, dtype=t.dtype, device=t.device)
+    dq = new(q) if want[0] or want[3] else None
+    dk = new(k) if want[1] or want[3] else None
+    dv = new(v) if want[2] or want[4] else None
+    per_token = log_decay.dim() == 3
+    dg = torch.empty(log_decay.shape, dtype=torch.float32, device=q.device) if want[3] else None
+    dh0 = torch.empty(B, heads, K, V, dtype=torch.float32, device=q.device) if want[4] else None
+    if B == 0 and dg is not None:
+        dg.zero_()
+    p = _problem(q, k, v, log_decay, lengths, h0, scale, heads, T)
+    scratch = _scratch(p, 2 if want[3] else 1, q.device)
+    ctx, g = workspace.call_context(q.device, scratch), _heads(grad_o)
+    views = [_heads(t) if t is not None else None for t in (dq, dk, dv)]
+    refs = [ctypes.byref(x) if x is not None else None for x in views]
+    _lib.check(_lib.lib().fss_linear_attention_backward(ctypes.byref(ctx), ctypes.byref(p), ctypes.byref(g), _pointer(h_last), _pointer(grad_last),
+                                                        *refs, _pointer(dg), int(per_token), _pointer(dh0)),
+               "fss_linear_attention_backward")
+    return [x if w else None for x, w in zip((dq, dk, dv, dg, dh0), want)]
+
+
+class LinearAttention(Function):
+    """Inputs: q, k, v, log_decay, h0 (or None), lengths (or None), scale, return the last state."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, log_decay, h0, lengths, scale: float, want_final: bool):
+        state = h0.detach().float().contiguous() if h0 is not None else None
+        o, h_last = linear_attention_forward(q, k, v, log_decay, scale=scale, h0=state, lengths=lengths, want_final=want_final)
+        ctx.set_materialize_grads(False)
+        ctx.scale = scale
+        ctx.h0_dtype = h0.dtype if h0 is not None else None
+        ctx.save_for_backward(q, k, v, log_decay, state, lengths, h_last if log_decay.requires_grad else None)
+        return (o, h_last) if want_final else o
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_o, grad_last=None):
+        q, k, v, log_decay, h0, lengths, h_last = ctx.saved_tensors
+        heads = max(q.shape[2], k.shape[2], v.shape[2])
+        if grad_o is None:
+            grad_o = torch.zeros(*q.shape[:2], heads, v.shape[3], dtype=v.dtype, device=v.device)
+        if grad_last is not None:
+            grad_last = grad_last.float().contiguous()
+        dq, dk, dv, dg, dh0 = linear_attention_backward(q, k, v, log_decay, grad_o.to(v.dtype), scale=ctx.scale, h0=h0, lengths=lengths,
+                                                        h_last=h_last, grad_last=grad_last, want=ctx.needs_input_grad[:5])
+        return dq, dk, dv, dg, dh0.to(ctx.h0_dtype) if dh0 is not None else None, None, None, None
+
+
+def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, *, scale: Optional[float] = None,
+                     h0: Optional[torch.Tensor] = None, return_final_state: bool = False, lengths: Optional[torch.Tensor] = None):
+    """Outputs ``[batch, seq, heads, value_dim]`` of whole sequences; with ``return_final_state`` also the fp32 state
+    behind the last token, ``[batch, heads, key_dim, value_dim]``, which continues the sequence as the next call's
+    ``h0``.  ``scale``: ``key_dim ** -0.5`` unless given.  See the module's docstring for layouts, decays and lengths."""
+    heads, K, V = _check_heads(q, k, v, log_decay, True)
+    B, T = q.shape[:2]
+    if h0 is not None:
+        _check("h0", h0, 4, q)
+        if h0.shape != (B, heads, K, V) or not h0.is_floating_point():
+            raise RuntimeError(f"h0: expected a floating-point [{B}, {heads}, {K}, {V}] tensor, got {h0.dtype} {list(h0.shape)}")
+    if lengths is not None:
+        _check("lengths", lengths, 1, q, torch.int32)
+        if lengths.shape != (B,):
+            raise RuntimeError(f"lengths: expected [{B}], got {list(lengths.shape)}")
+        lengths = lengths.contiguous()
+    scale = K ** -0.5 if scale is None else float(scale)
+    needs = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or log_decay.requires_grad
+                                         or (h0 is not None and h0.requires_grad))
+    if needs:
+        return LinearAttention.apply(q, k, v, log_decay, h0, lengths, scale, bool(return_final_state))
+    state = h0.detach().float().contiguous() if h0 is not None else None
+    o, h_last = linear_attention_forward(q, k, v, log_decay, scale=scale, h0=state, lengths=lengths, want_final=bool(return_final_state))
+    return (o, h_last) if return_final_state else o
+
+
+def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, state: torch.Tensor, *,
+                          scale: Optional[float] = None, slots: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """One token for each sequence: ``q, k, v`` ``[batch, heads, dim]``, ``log_decay`` ``[heads]`` or ``[batch, heads]``;
+    returns ``o`` ``[batch, heads, value_dim]`` and updates ``state`` in place.
+
+    ``state``: fp32 ``[pool, heads, key_dim, value_dim]`` with contiguous states; sequence ``b`` has the entry ``slots[b]``
+    (int32, on the device), or ``b`` without ``slots``.  A slot outside the pool (-1, say) marks a row of padding: its
+    output is zeros and no state is touched.  Two sequences of a call must not share a slot.  Not differentiable."""
+    heads, K, V = _check_heads(q, k, v, log_decay, False)
+    B = q.shape[0]
+    _check("state", state, 4, q, torch.float32)
+    if state.shape[1:] != (heads, K, V):
+        raise RuntimeError(f"state: expected [pool, {heads}, {K}, {V}], got {list(state.shape)}")
+    if state.numel() and not state[0].is_contiguous():
+        raise RuntimeError("state: each sequence's states have to be contiguous")
+    if state.shape[0] > 1 and state.numel() and state.stride(0) < heads * K * V:
+        raise RuntimeError("state: the sequences' states overlap")
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, log_decay, state)):
+        raise RuntimeError("linear_attention_step is not differentiable: use linear_attention, or torch.no_grad()")
+    if slots is not None:
+        _check("slots", slots, 1, q, torch.int32)
+        if slots.shape != (B,):
+            raise RuntimeError(f"slots: expected [{B}], got {list(slots.shape)}")
+        slots = slots.contiguous()
+    elif state.shape[0] < B:
+        raise RuntimeError(f"state: {state.shape[0]} entries for {B} sequences")
+    scale = K ** -0.5 if scale is None else float(scale)
+    q, k, v = _channels(q), _channels(k), _channels(v)
+    o = torch.empty(B, heads, V, dtype=v.dtype, device=v.device)
+    p, out = _problem(q, k, v, log_decay, None, None, scale, heads, 1), _heads(o)
+    ctx = workspace.call_context(v.device)
+    _lib.check(_lib.lib().fss_linear_attention_step(ctypes.byref(ctx), ctypes.byref(p), ctypes.byref(out), state.data_ptr(), state.stride(0),
+                                                    state.shape[0], _pointer(slots)), "fss_linear_attention_step")
+    return o

@@ -18,6 +18,7 @@ from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
+OBJECTS = PKG / "build"      # one object for each .cu, with the list of what it was made from
 LIB = PKG / "libfss_b200.so"
 TORCH_SOURCE = CSRC / "fss_torch.cpp"
 
@@ -26,7 +27,6 @@ NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-lineinfo",
     "-Xcompiler", "-fPIC,-fvisibility=hidden",
-    "-shared",
 ]
 
 
@@ -75,19 +75,38 @@ def build_torch(force: bool = False) -> Path:
     return lib
 
 
+def _object_is_stale(source: Path, obj: Path) -> bool:
+    made_from = obj.with_suffix(".d")
+    if not obj.is_file() or not made_from.is_file():
+        return True
+    t = obj.stat().st_mtime
+    names = made_from.read_text().replace("\\\n", " ").split(":", 1)[-1].split()
+    return any(not Path(n).is_file() or Path(n).stat().st_mtime > t for n in [str(source), str(Path(__file__)), *names])
+
+
+def _compile(nvcc: str, source: Path, obj: Path, verbose: bool):
+    cmd = [nvcc, *NVCC_FLAGS, *(["-Xptxas", "-v"] if verbose else []), "-MD", "-MF", str(obj.with_suffix(".d")), "-c", str(source), "-o", str(obj)]
+    return subprocess.run(cmd, env=dict(os.environ), capture_output=True, text=True)
+
+
 def build(force: bool = False, verbose: bool = False) -> Path:
     build_torch(force)
     if not force and not is_stale():
         return LIB
-    cmd = [_nvcc(), *NVCC_FLAGS]
-    if verbose:
-        cmd += ["-Xptxas", "-v"]
-    cmd += ["-o", str(LIB)] + [str(f) for f in sorted(CSRC.glob("*.cu"))]
-    env = dict(os.environ)
-    res = subprocess.run(cmd, env=env, capture_output=True, text=True)
-    if verbose or res.returncode:
-        sys.stderr.write(res.stdout + res.stderr)
-    if res.returncode:
+    from concurrent.futures import ThreadPoolExecutor
+    nvcc = _nvcc()
+    OBJECTS.mkdir(exist_ok=True)
+    objects = {f: OBJECTS / f"{f.stem}.o" for f in sorted(CSRC.glob("*.cu"))}
+    stale = [f for f, o in objects.items() if force or _object_is_stale(f, o)]
+    with ThreadPoolExecutor(len(objects)) as pool:
+        results = list(pool.map(lambda f: _compile(nvcc, f, objects[f], verbose), stale))
+    if not any(r.returncode for r in results):
+        results.append(subprocess.run([nvcc, *NVCC_FLAGS, "-shared", "-o", str(LIB), *map(str, objects.values())], capture_output=True, text=True))
+    failed = any(r.returncode for r in results)
+    if verbose or failed:
+        for r in results:
+            sys.stderr.write(r.stdout + r.stderr)
+    if failed:
         raise RuntimeError("nvcc failed building libfss_b200.so")
     return LIB
 

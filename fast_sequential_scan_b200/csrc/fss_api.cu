@@ -9,11 +9,10 @@
 #include "fss_chunked.cuh"
 #include "fss_common.cuh"
 #include "fss_gates.cuh"
+#include "fss_host.cuh"
 #include "fss_lookback.cuh"
 #include "fss_ragged.cuh"
 #include "fss_seqpar.cuh"
-
-#define FSS_API extern "C" __attribute__((visibility("default")))
 
 namespace fss {
 
@@ -23,43 +22,6 @@ thread_local std::string g_cuda_error;
 int cuda_fail(cudaError_t e, const char *what, int code) {
     g_cuda_error = std::string(what) + ": " + cudaGetErrorName(e) + " (" + cudaGetErrorString(e) + ")";
     return code;
-}
-
-#define FSS_CUDA(call, what)                                      \
-    do {                                                          \
-        cudaError_t e_ = (call);                                  \
-        if (e_ != cudaSuccess) return cuda_fail(e_, what, FSS_E_LAUNCH); \
-    } while (0)
-
-// Makes ctx->device current for the duration of a call and puts the previous one back.  The
-// first call of a thread always binds the device, so that driver entry points used later (TMA
-// descriptor encoding) find a current context even on threads that never touched CUDA through
-// this library (autograd worker threads, for instance).
-struct DeviceGuard {
-    int prev = -1;
-    bool switched = false;
-    int error = FSS_OK;
-    int device = -1;
-    explicit DeviceGuard(int want) {
-        static thread_local int bound = -1;
-        cudaError_t e = cudaGetDevice(&prev);
-        if (e != cudaSuccess) { error = cuda_fail(e, "cudaGetDevice", FSS_E_DEVICE); return; }
-        device = want >= 0 ? want : prev;
-        if (device != prev || bound != device) {
-            e = cudaSetDevice(device);
-            if (e != cudaSuccess) { error = cuda_fail(e, "cudaSetDevice", FSS_E_DEVICE); return; }
-            bound = device;
-            switched = device != prev;
-        }
-    }
-    ~DeviceGuard() { if (switched) cudaSetDevice(prev); }
-};
-
-static int check_ctx(const fss_scan_ctx *ctx) {
-    if (!ctx) return FSS_E_NULL;
-    if (ctx->struct_bytes != sizeof(fss_scan_ctx)) return FSS_E_ARGS;
-    if (ctx->algo < FSS_ALGO_AUTO || ctx->algo > FSS_ALGO_LOOKBACK) return FSS_E_ALGO;
-    return FSS_OK;
 }
 
 static int check_view(const fss_view *v, int64_t B, int64_t T, int64_t D) {
@@ -88,11 +50,6 @@ static int need_workspace(const fss_scan_ctx *ctx, int64_t B, int64_t T, int64_t
     if (!ctx->workspace || ctx->workspace_bytes < fss_workspace_bytes(B, T, D, dtype)) return FSS_E_WORKSPACE;
     if (!aligned16(ctx->workspace)) return FSS_E_WORKSPACE;
     return FSS_OK;
-}
-
-static int launch_check(const char *what) {
-    cudaError_t e = cudaGetLastError();
-    return e == cudaSuccess ? FSS_OK : cuda_fail(e, what, FSS_E_LAUNCH);
 }
 
 // ------------------------------------------------------------------ chunked path

@@ -1,0 +1,64 @@
+// Host side of the C entry points, shared by the library's translation units: errors, the current device, checks.
+#pragma once
+
+#include "fss_common.cuh"
+
+#define FSS_API extern "C" __attribute__((visibility("default")))
+
+namespace fss {
+
+#define FSS_CUDA(call, what)                                      \
+    do {                                                          \
+        cudaError_t e_ = (call);                                  \
+        if (e_ != cudaSuccess) return cuda_fail(e_, what, FSS_E_LAUNCH); \
+    } while (0)
+
+// Makes ctx->device current for the duration of a call and puts the previous one back.  The
+// first call of a thread always binds the device, so that driver entry points used later (TMA
+// descriptor encoding) find a current context even on threads that never touched CUDA through
+// this library (autograd worker threads, for instance).
+struct DeviceGuard {
+    int prev = -1;
+    bool switched = false;
+    int error = FSS_OK;
+    int device = -1;
+    explicit DeviceGuard(int want) {
+        static thread_local int bound = -1;
+        cudaError_t e = cudaGetDevice(&prev);
+        if (e != cudaSuccess) { error = cuda_fail(e, "cudaGetDevice", FSS_E_DEVICE); return; }
+        device = want >= 0 ? want : prev;
+        if (device != prev || bound != device) {
+            e = cudaSetDevice(device);
+            if (e != cudaSuccess) { error = cuda_fail(e, "cudaSetDevice", FSS_E_DEVICE); return; }
+            bound = device;
+            switched = device != prev;
+        }
+    }
+    ~DeviceGuard() { if (switched) cudaSetDevice(prev); }
+};
+
+inline int check_ctx(const fss_scan_ctx *ctx) {
+    if (!ctx) return FSS_E_NULL;
+    if (ctx->struct_bytes != sizeof(fss_scan_ctx)) return FSS_E_ARGS;
+    if (ctx->algo < FSS_ALGO_AUTO || ctx->algo > FSS_ALGO_LOOKBACK) return FSS_E_ALGO;
+    return FSS_OK;
+}
+
+inline int launch_check(const char *what) {
+    cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? FSS_OK : cuda_fail(e, what, FSS_E_LAUNCH);
+}
+
+// multiprocessors of the current device (cached per device; 148 if the query fails)
+inline int multiprocessors() {
+    static int cached[64] = {0};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+    if (cached[dev] == 0) {
+        int n = 0;
+        cached[dev] = (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess && n > 0) ? n : 148;
+    }
+    return cached[dev];
+}
+
+}  // namespace fss

@@ -1,0 +1,287 @@
+// C entry points of linear attention (include/fss_b200.h): argument checks, plans, launches.
+#include "fss_host.cuh"
+#include "fss_linattn.cuh"
+
+namespace fss {
+namespace linattn {
+
+static int check_heads(const fss_heads *x, int64_t B, int64_t T, int64_t H, int64_t dim) {
+    if (x->heads < 1 || H % x->heads || x->dim != dim) return FSS_E_SHAPE;
+    if (x->stride_b < 0 || x->stride_t < 0 || x->stride_h < 0) return FSS_E_SHAPE;
+    if (B * T > 0 && !x->ptr) return FSS_E_NULL;
+    if (B > 1 && x->stride_b > (INT64_MAX / 32) / B) return FSS_E_SHAPE;
+    if (T > 1 && x->stride_t > (INT64_MAX / 32) / T) return FSS_E_SHAPE;
+    if (x->heads > 1 && x->stride_h > (INT64_MAX / 32) / x->heads) return FSS_E_SHAPE;
+    return FSS_OK;
+}
+// an output's elements must not share memory
+static int check_output(const fss_heads *x, int64_t B, int64_t T, int64_t H, int64_t dim) {
+    const int rc = check_heads(x, B, T, H, dim);
+    if (rc) return rc;
+    if (x->heads > 1 && x->stride_h < dim) return FSS_E_SHAPE;
+    if (T > 1 && x->stride_t < (x->heads - 1) * x->stride_h + dim) return FSS_E_SHAPE;
+    if (B > 1 && x->stride_b < (T - 1) * x->stride_t + (x->heads - 1) * x->stride_h + dim) return FSS_E_SHAPE;
+    return FSS_OK;
+}
+
+static int check_problem(const fss_linear_attention *p) {
+    if (!p) return FSS_E_NULL;
+    if (p->struct_bytes != sizeof(fss_linear_attention)) return FSS_E_ARGS;
+    if (p->dtype != FSS_DTYPE_BF16 && p->dtype != FSS_DTYPE_F32) return FSS_E_DTYPE;
+    if (p->B < 0 || p->T < 0 || p->H < 1 || p->T > INT32_MAX) return FSS_E_SHAPE;
+    if (p->q.dim < 1 || p->v.dim < 1) return FSS_E_SHAPE;
+    if (p->q.dim > kMaxDim || p->v.dim > kMaxDim) return FSS_E_TOO_LARGE;
+    if (p->B > 0 && p->H > (INT64_MAX / (8 * kMaxDim * kMaxDim)) / p->B) return FSS_E_SHAPE;
+    if (p->B > 0 && p->T > 0 && p->B * p->H > (INT64_MAX / (8 * kMaxDim)) / p->T) return FSS_E_SHAPE;
+    int rc;
+    if ((rc = check_heads(&p->q, p->B, p->T, p->H, p->q.dim))) return rc;
+    if ((rc = check_heads(&p->k, p->B, p->T, p->H, p->q.dim))) return rc;
+    if ((rc = check_heads(&p->v, p->B, p->T, p->H, p->v.dim))) return rc;
+    if (p->B > 0 && !p->log_decay) return FSS_E_NULL;
+    if (p->decay_stride_b < 0 || p->decay_stride_t < 0 || p->decay_stride_h < 0) return FSS_E_SHAPE;
+    return FSS_OK;
+}
+
+// ------------------------------------------------------------------ plans
+struct Plan {
+    int lanes, warps, v_tiles, nseg;
+    int64_t seg_len;
+    size_t seg_bytes;      // states and decays of the segments
+};
+
+// One pass over tensors of key dimension Dk and value dimension Dv.
+static Plan make_plan(int64_t B, int64_t T, int64_t H, int64_t Dk, int64_t Dv) {
+    Plan w{};
+    w.lanes = Dk <= 32 ? 1 : Dk <= 64 ? 2 : Dk <= 128 ? 4 : 8;
+    const int64_t columns = 32 / w.lanes * kLaneV;
+    w.warps = (int)(ceil_div(Dv, columns) < 4 ? ceil_div(Dv, columns) : 4);
+    w.v_tiles = (int)ceil_div(Dv, columns * w.warps);
+    // two CTAs of four warps a multiprocessor (registers); a pass for the sums alone does two thirds of the work
+    w.nseg = choose_segments(B * H * w.v_tiles, T, kPlannedSms * (8 / w.warps), kBlock, 0.67, 4.0);
+    w.seg_len = ceil_div(ceil_div(T > 0 ? T : 1, kBlock), w.nseg) * kBlock;
+    w.seg_bytes = w.nseg > 1 ? align_up((size_t)(B * H * w.nseg) * (size_t)(Dk * Dv + 1) * sizeof(float), 256) : 0;
+    return w;
+}
+
+template <typename T> static bool wide_rows(const Heads<const T> &x, int D) {
+    constexpr int64_t V = VecWidth<T>::value;
+    return aligned16(x.ptr) && D % V == 0 && x.sb % V == 0 && x.st % V == 0 && x.sh % V == 0;
+}
+
+// ------------------------------------------------------------------ launches
+struct Pass {
+    fss_heads q, k, v;
+    float in_scale, out_scale;
+    bool reverse, transposed;      // transposed: state_in and state_out hold [Dv, Dk]
+    const float *state_in;
+    float *state_out;
+};
+
+static Problem make_problem(const fss_linear_attention *p, const Pass &s, const Plan &w, void *scratch) {
+    Problem x{};
+    x.B = p->B; x.T = p->T; x.H = p->H;
+    x.Dk = (int)s.q.dim; x.Dv = (int)s.v.dim;
+    x.g = p->log_decay;
+    x.gsb = p->decay_stride_b; x.gst = p->decay_stride_t; x.gsh = p->decay_stride_h;
+    x.lengths = p->lengths;
+    x.in_scale = s.in_scale; x.out_scale = s.out_scale;
+    x.reverse = s.reverse;
+    x.state_in = s.state_in; x.state_out = s.state_out;
+    x.sk = s.transposed ? 1 : x.Dv;
+    x.sv = s.transposed ? x.Dk : 1;
+    x.nseg = w.nseg; x.seg_len = w.seg_len;
+    x.seg_state = static_cast<float *>(scratch);
+    x.seg_decay = x.seg_state + x.B * x.H * w.nseg * (int64_t)x.Dk * x.Dv;
+    return x;
+}
+
+template <typename T, typename TO, int L> static int run_recurrent(const Problem &x, const Plan &w, const Pass &s, const fss_heads *o, cudaStream_t stream) {
+    const auto q = make_heads<const T>(&s.q, x.H), k = make_heads<const T>(&s.k, x.H), v = make_heads<const T>(&s.v, x.H);
+    const auto out = make_heads<TO>(o, x.H);
+    const int vec = wide_rows(q, x.Dk) && wide_rows(k, x.Dk) && wide_rows(v, x.Dv);
+    const int64_t blocks = x.B * x.H * w.nseg * w.v_tiles;
+    if (blocks > INT32_MAX) return FSS_E_SHAPE;
+    const size_t smem = shared_bytes<L>(w.warps);
+    auto *sums = recurrent<T, TO, L, false>;
+    auto *outputs = recurrent<T, TO, L, true>;
+    if (smem > 48 * 1024) {
+        FSS_CUDA(cudaFuncSetAttribute(sums, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), "shared memory of a recurrent pass");
+        FSS_CUDA(cudaFuncSetAttribute(outputs, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), "shared memory of a recurrent pass");
+    }
+    if (w.nseg > 1) {
+        sums<<<(unsigned)blocks, w.warps * 32, smem, stream>>>(x, q, k, v, out, w.v_tiles, vec);
+        fold_segments<<<(unsigned)(x.B * x.H * ceil_div((int64_t)x.Dk * x.Dv, 256)), 256, 0, stream>>>(x);
+    }
+    outputs<<<(unsigned)blocks, w.warps * 32, smem, stream>>>(x, q, k, v, out, w.v_tiles, vec);
+    return launch_check("linear attention launch");
+}
+
+template <typename T, typename TO> static int run_pass(const fss_linear_attention *p, const Pass &s, const fss_heads *o, void *scratch, cudaStream_t stream) {
+    const Plan w = make_plan(p->B, p->T, p->H, s.q.dim, s.v.dim);
+    const Problem x = make_problem(p, s, w, scratch);
+    if (w.lanes == 1) return run_recurrent<T, TO, 1>(x, w, s, o, stream);
+    if (w.lanes == 2) return run_recurrent<T, TO, 2>(x, w, s, o, stream);
+    if (w.lanes == 4) return run_recurrent<T, TO, 4>(x, w, s, o, stream);
+    return run_recurrent<T, TO, 8>(x, w, s, o, stream);
+}
+
+// ------------------------------------------------------------------ gradients
+struct BackwardPlan {
+    size_t seg, each, dots, sums;      // bytes
+    bool dq_each, dk_each, dv_each;
+};
+static BackwardPlan plan_backward(const fss_linear_attention *p, bool decays) {
+    BackwardPlan w{};
+    const int64_t n = p->B * p->T * p->H, Dk = p->q.dim, Dv = p->v.dim;
+    const size_t a = make_plan(p->B, p->T, p->H, Dv, Dk).seg_bytes, b = make_plan(p->B, p->T, p->H, Dk, Dv).seg_bytes;
+    w.seg = a > b ? a : b;
+    w.dq_each = decays || p->q.heads < p->H;
+    w.dk_each = decays || p->k.heads < p->H;
+    w.dv_each = p->v.heads < p->H;
+    const int64_t widest = (w.dq_each || w.dk_each) && (Dk > Dv || !w.dv_each) ? Dk : w.dv_each ? Dv : 0;
+    w.each = align_up((size_t)(n * widest) * sizeof(float), 256);
+    w.dots = decays ? align_up((size_t)n * sizeof(float), 256) : 0;
+    w.sums = decays ? align_up((size_t)(p->B * p->H) * sizeof(float), 256) : 0;
+    return w;
+}
+
+// One of the three gradients: straight to its tensor, or by way of fp32 copies for each state.
+template <typename T>
+static int run_gradient(const fss_linear_attention *p, const Pass &s, const fss_heads &x, const fss_heads *dx, bool by_state, float *each, float *dots,
+                        void *scratch, cudaStream_t stream) {
+    if (!by_state) return run_pass<T, T>(p, s, dx, scratch, stream);
+    const int64_t D = s.v.dim;
+    const fss_heads o{each, p->T * p->H * D, p->H * D, D, p->H, D};
+    const int rc = run_pass<T, float>(p, s, &o, scratch, stream);
+    if (rc) return rc;
+    const int64_t blocks = ceil_div(p->B * p->T * x.heads, 8);
+    if (blocks > INT32_MAX) return FSS_E_SHAPE;
+    finish_gradient<T><<<(unsigned)blocks, 256, 0, stream>>>(p->B, p->T, p->H, x.heads, (int)D, each, make_heads<const T>(&x, p->H), make_heads<T>(dx, p->H), dots);
+    return launch_check("linear attention gradient launch");
+}
+
+template <typename T>
+static int run_backward(const fss_scan_ctx *ctx, const fss_linear_attention *p, const fss_heads *grad_o, const float *h_last, const float *grad_last,
+                        const fss_heads *dq, const fss_heads *dk, const fss_heads *dv, float *grad_decay, int per_token, float *grad_h0) {
+    cudaStream_t stream = (cudaStream_t)ctx->stream;
+    const BackwardPlan w = plan_backward(p, grad_decay != nullptr);
+    char *at = static_cast<char *>(ctx->workspace);
+    void *scratch = at;
+    float *each = reinterpret_cast<float *>(at + w.seg);
+    float *q_dq = w.dots ? reinterpret_cast<float *>(at + w.seg + w.each) : nullptr;
+    float *k_dk = w.dots ? reinterpret_cast<float *>(at + w.seg + w.each + w.dots) : nullptr;
+    float *sums = w.dots ? reinterpret_cast<float *>(at + w.seg + w.each + 2 * w.dots) : nullptr;
+    int rc;
+    if (dq || grad_decay) {
+        const Pass s{*grad_o, p->v, p->k, 1.f, p->scale, false, true, p->h0, nullptr};
+        if ((rc = run_gradient<T>(p, s, p->q, dq, w.dq_each, each, q_dq, scratch, stream))) return rc;
+    }
+    if (dk || grad_decay) {
+        const Pass s{p->v, *grad_o, p->q, p->scale, 1.f, true, true, grad_last, nullptr};
+        if ((rc = run_gradient<T>(p, s, p->k, dk, w.dk_each, each, k_dk, scratch, stream))) return rc;
+    }
+    if (dv || grad_h0) {
+        const Pass s{p->k, p->q, *grad_o, p->scale, 1.f, true, false, grad_last, grad_h0};
+        if ((rc = run_gradient<T>(p, s, p->v, dv, w.dv_each, each, nullptr, scratch, stream))) return rc;
+    }
+    if (grad_decay) {
+        Problem x{};
+        x.B = p->B; x.T = p->T; x.H = p->H;
+        x.Dk = (int)p->q.dim; x.Dv = (int)p->v.dim;
+        x.g = p->log_decay;
+        x.gsb = p->decay_stride_b; x.gst = p->decay_stride_t; x.gsh = p->decay_stride_h;
+        x.lengths = p->lengths;
+        decay_gradient<<<(unsigned)(p->B * p->H), kFlowThreads, 0, stream>>>(x, q_dq, k_dk, h_last, grad_last, per_token ? grad_decay : nullptr,
+                                                                              per_token ? nullptr : sums);
+        if (!per_token) sum_sequences<<<(unsigned)ceil_div(p->H, 128), 128, 0, stream>>>(p->B, p->H, sums, grad_decay);
+        return launch_check("decay gradient launch");
+    }
+    return FSS_OK;
+}
+
+}  // namespace linattn
+}  // namespace fss
+
+using namespace fss;
+using namespace fss::linattn;
+
+static bool big_enough(const fss_scan_ctx *ctx, size_t need) {
+    return need == 0 || (ctx->workspace && ctx->workspace_bytes >= need && aligned16(ctx->workspace));
+}
+
+FSS_API size_t fss_linear_attention_workspace_bytes(const fss_linear_attention *p, int backward) {
+    if (check_problem(p) || p->B == 0) return 0;
+    if (!backward) return make_plan(p->B, p->T, p->H, p->q.dim, p->v.dim).seg_bytes;
+    const BackwardPlan w = plan_backward(p, backward > 1);
+    return w.seg + w.each + 2 * w.dots + w.sums;
+}
+
+FSS_API int fss_linear_attention_forward(const fss_scan_ctx *ctx, const fss_linear_attention *p, const fss_heads *o, float *h_last) {
+    int rc;
+    if ((rc = check_ctx(ctx)) || (rc = check_problem(p))) return rc;
+    if (!o) return FSS_E_NULL;
+    if ((rc = check_output(o, p->B, p->T, p->H, p->v.dim))) return rc;
+    if (o->heads != p->H) return FSS_E_SHAPE;
+    if (p->B == 0 || (p->T == 0 && !h_last)) return FSS_OK;
+    if (!big_enough(ctx, fss_linear_attention_workspace_bytes(p, 0))) return FSS_E_WORKSPACE;
+    DeviceGuard guard(ctx->device);
+    if (guard.error) return guard.error;
+    const Pass s{p->q, p->k, p->v, 1.f, p->scale, false, false, p->h0, h_last};
+    return p->dtype == FSS_DTYPE_BF16 ? run_pass<bf16, bf16>(p, s, o, ctx->workspace, (cudaStream_t)ctx->stream)
+                                      : run_pass<float, float>(p, s, o, ctx->workspace, (cudaStream_t)ctx->stream);
+}
+
+FSS_API int fss_linear_attention_backward(const fss_scan_ctx *ctx, const fss_linear_attention *p, const fss_heads *grad_o, const float *h_last,
+                                          const float *grad_last, const fss_heads *dq, const fss_heads *dk, const fss_heads *dv, float *grad_decay,
+                                          int per_token, float *grad_h0) {
+    int rc;
+    if ((rc = check_ctx(ctx)) || (rc = check_problem(p))) return rc;
+    if (!grad_o || (grad_decay && grad_last && !h_last)) return FSS_E_NULL;
+    if ((rc = check_heads(grad_o, p->B, p->T, p->H, p->v.dim)) || grad_o->heads != p->H) return rc ? rc : FSS_E_SHAPE;
+    // the decays' gradients are made of those of queries and keys, the first state's is a by-product of the values'
+    if ((grad_decay && !(dq && dk)) || (grad_h0 && !dv)) return FSS_E_NULL;
+    if (dq && ((rc = check_output(dq, p->B, p->T, p->H, p->q.dim)) || dq->heads != p->q.heads)) return rc ? rc : FSS_E_SHAPE;
+    if (dk && ((rc = check_output(dk, p->B, p->T, p->H, p->q.dim)) || dk->heads != p->k.heads)) return rc ? rc : FSS_E_SHAPE;
+    if (dv && ((rc = check_output(dv, p->B, p->T, p->H, p->v.dim)) || dv->heads != p->v.heads)) return rc ? rc : FSS_E_SHAPE;
+    if (p->B == 0) return FSS_OK;
+    if (!big_enough(ctx, fss_linear_attention_workspace_bytes(p, grad_decay ? 2 : 1))) return FSS_E_WORKSPACE;
+    DeviceGuard guard(ctx->device);
+    if (guard.error) return guard.error;
+    return p->dtype == FSS_DTYPE_BF16 ? run_backward<bf16>(ctx, p, grad_o, h_last, grad_last, dq, dk, dv, grad_decay, per_token, grad_h0)
+                                      : run_backward<float>(ctx, p, grad_o, h_last, grad_last, dq, dk, dv, grad_decay, per_token, grad_h0);
+}
+
+template <typename T>
+static int run_step(const fss_scan_ctx *ctx, const fss_linear_attention *p, const fss_heads *o, float *states, int64_t stride, int64_t pool, const int32_t *slots) {
+    const int Dk = (int)p->q.dim, Dv = (int)p->v.dim;
+    const bool wide = Dv % 4 == 0 && stride % 4 == 0 && aligned16(states);
+    const int V = wide ? 4 : 1;
+    // 64 columns a CTA: with 128 threads eight rows of a wide state at a time
+    int columns = 64 < Dv ? 64 : Dv;
+    if (!wide && columns > kStepThreads) columns = kStepThreads;
+    const int tiles = (int)ceil_div(Dv, columns);
+    const int64_t blocks = p->B * p->H * tiles;
+    if (blocks > INT32_MAX) return FSS_E_SHAPE;
+    const auto q = make_heads<const T>(&p->q, p->H), k = make_heads<const T>(&p->k, p->H), v = make_heads<const T>(&p->v, p->H);
+    const auto out = make_heads<T>(o, p->H);
+    auto *kernel = V == 4 ? step<T, 4> : step<T, 1>;
+    kernel<<<(unsigned)blocks, kStepThreads, 0, (cudaStream_t)ctx->stream>>>(p->B, p->H, Dk, Dv, q, k, v, out, p->log_decay, p->decay_stride_b, p->decay_stride_h,
+                                                                             p->scale, states, stride, pool, slots, tiles, columns);
+    return launch_check("linear attention step launch");
+}
+
+FSS_API int fss_linear_attention_step(const fss_scan_ctx *ctx, const fss_linear_attention *p, const fss_heads *o, float *states, int64_t state_stride,
+                                      int64_t pool, const int32_t *slots) {
+    int rc;
+    if ((rc = check_ctx(ctx)) || (rc = check_problem(p))) return rc;
+    if (!o || (p->B > 0 && pool > 0 && !states)) return FSS_E_NULL;
+    if (p->T != 1 || p->lengths || p->h0) return FSS_E_ARGS;
+    if ((rc = check_output(o, p->B, 1, p->H, p->v.dim)) || o->heads != p->H) return rc ? rc : FSS_E_SHAPE;
+    if (pool < 0 || (!slots && pool < p->B) || (pool > 1 && state_stride < p->H * p->q.dim * p->v.dim)) return FSS_E_SHAPE;
+    if (pool > 1 && state_stride > (INT64_MAX / 8) / pool) return FSS_E_SHAPE;
+    if (p->B == 0) return FSS_OK;
+    DeviceGuard guard(ctx->device);
+    if (guard.error) return guard.error;
+    return p->dtype == FSS_DTYPE_BF16 ? run_step<bf16>(ctx, p, o, states, state_stride, pool, slots)
+                                      : run_step<float>(ctx, p, o, states, state_stride, pool, slots);
+}

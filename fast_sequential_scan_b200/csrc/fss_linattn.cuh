@@ -1,0 +1,507 @@
+// Linear attention with a decay for each head: the recurrence of this library with a matrix for a state,
+//
+//     S_t = e^{g_t} S_{t-1} + k_t v_t^T ,      o_t = q_t^T S_t          S: [Dk, Dv] fp32 for each (sequence, head)
+//
+// "Visiting order": the kernels walk the valid tokens 0 .. len-1 of a sequence forwards, or, for the gradients, from
+// len-1 to 0 with the adjoint's decays (visiting t multiplies the state by e^{g_{t+1}}, the first visit by 1):
+//
+//     dq = LA(q: do, k: v, v: k)  forwards, state S^T        dk = LA(q: v, k: do, v: q)  backwards, state R^T
+//     dv = LA(q: k, k: q, v: do)  backwards, state R         R_t = e^{g_{t+1}} R_{t+1} + q_t do_t^T
+//
+// so that one operator serves the forward and its three gradients.  Rows from len to T are never read; their outputs
+// are zeros.
+//
+// A long sequence is cut into segments that run at the same time: a first launch takes every segment's own sum
+// (its state from an empty one) and decay, a second folds them in order into the state that enters each segment, a
+// third computes the outputs.  No CTA waits for another.
+//
+// This file: the definitions that all linear-attention kernels share, and the recurrent kernels, which take one token
+// after the other with the state in registers, in fp32 throughout: any head dimension up to 256, any strides, both
+// types.
+#pragma once
+
+#include "fss_common.cuh"
+
+namespace fss {
+namespace linattn {
+
+constexpr int kMaxDim = 256;      // of keys and values
+
+template <typename T> struct Heads {
+    T *ptr;
+    int64_t sb, st, sh;      // strides in elements
+    int64_t group;           // heads of the state that share one of this tensor
+    __host__ __device__ __forceinline__ T *row(int64_t b, int64_t t, int64_t h) const { return ptr + b * sb + t * st + (h / group) * sh; }
+};
+
+template <typename T> inline Heads<T> make_heads(const fss_heads *x, int64_t H) {
+    return Heads<T>{reinterpret_cast<T *>(x->ptr), x->stride_b, x->stride_t, x->stride_h, x->heads ? H / x->heads : 1};
+}
+
+struct Problem {
+    int64_t B, T, H;
+    int Dk, Dv;
+    const float *g;      // log decays
+    int64_t gsb, gst, gsh;
+    const int32_t *lengths;      // valid tokens of each sequence, or NULL: all T
+    float in_scale, out_scale;      // of k v^T, of the outputs
+    bool reverse;
+    const float *state_in;      // [B, H] matrices of Dk x Dv with the strides below, or NULL: empty
+    float *state_out;           // or NULL
+    int64_t sk, sv;
+    int nseg;
+    int64_t seg_len;         // tokens a segment
+    float *seg_state;        // [B, H, nseg] matrices [Dk, Dv]: a segment's own sum, later the state that enters it
+    float *seg_decay;        // [B, H, nseg]
+
+    __device__ __forceinline__ int64_t length(int64_t b) const {
+        if (!lengths) return T;
+        const int64_t n = lengths[b];
+        return n < 0 ? 0 : n > T ? T : n;
+    }
+    // the token of visit s; visits from len on are the rows that only get zeros
+    __device__ __forceinline__ int64_t token(int64_t s, int64_t len) const { return reverse && s < len ? len - 1 - s : s; }
+    // the logarithm of what visit s multiplies the state with before it adds its token (s < len)
+    __device__ __forceinline__ float log_decay(int64_t b, int64_t h, int64_t s, int64_t len) const {
+        const int64_t t = reverse ? len - s : s;
+        if (reverse && s == 0) return 0.f;
+        return g[b * gsb + t * gst + h * gsh];
+    }
+};
+
+// ------------------------------------------------------------------ recurrent kernels
+// One thread holds 32 x 4 elements of the state: 32 key channels of 4 value channels.  L lanes hold a value channel's
+// (up to 32 L) key channels between them, so the outputs' sums over the key channels take log2(L) shuffles.  Per token
+// and state element that is one multiplication and three fused multiply-adds, in packed pairs; keys and queries come
+// from shared memory, each 16 bytes of them for 16 state elements.  A decay comes in two parts, the fp32 value nearest to
+// it and what that leaves: the same decay multiplies the state thousands of times, and its rounding would come in as
+// often (2^-25 a token; 1e-4 over a memory of 4,096).
+//
+// Bound by the fp32 pipes: 4 Dk Dv operations a token against 2 (2 Dk + 2 Dv) or twice that many bytes.
+constexpr int kLaneK = 32, kLaneV = 4;
+constexpr int kBlock = 32;      // tokens staged in shared memory at a time (a warp's lanes take their decays)
+constexpr int kPitch = kLaneK + 4;                        // floats between the key channels of neighbouring lanes: other banks
+
+template <int L> struct Shape {
+    static constexpr int kColumns = 32 / L * kLaneV;      // value channels of a warp
+    static constexpr int kKeyRow = L * kPitch;
+};
+
+template <int L> inline size_t shared_bytes(int warps) {
+    return (size_t)kBlock * (2 * Shape<L>::kKeyRow + warps * Shape<L>::kColumns + 2) * sizeof(float);
+}
+
+// rows of `n` channels (zeros up to `padded`) into shared memory as fp32; key rows are laid out in lane order
+template <typename T, bool kKeys>
+__device__ __forceinline__ void stage(float *to, int pitch, const Heads<const T> &x, const Problem &p, int64_t b, int64_t h, int64_t first, int rows,
+                                      int64_t len, int offset, int n, int padded, float scale, bool vec) {
+    constexpr int V = VecWidth<T>::value;
+    const int per_row = padded / V;
+    for (int i = threadIdx.x; i < rows * per_row; i += blockDim.x) {
+        const int r = i / per_row, c = i % per_row * V;
+        const T *row = x.row(b, p.token(first + r, len), h) + offset;
+        float f[V];
+        if (vec && c + V <= n) {
+            Frag<T, V>::load(row + c, f);
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; ++j) f[j] = c + j < n ? (float)row[c + j] : 0.f;
+        }
+        float *at = to + r * pitch + (kKeys ? c / kLaneK * kPitch + c % kLaneK : c);
+#pragma unroll
+        for (int j = 0; j < V; j += 4) *reinterpret_cast<float4 *>(at + j) = make_float4(f[j] * scale, f[j + 1] * scale, f[j + 2] * scale, f[j + 3] * scale);
+    }
+}
+
+// kOut: outputs (and the last state, where there is one segment); else the segments' own sums.
+template <typename T, typename TO, int L, bool kOut>
+__global__ void __launch_bounds__(128) recurrent(Problem p, Heads<const T> q, Heads<const T> k, Heads<const T> v, Heads<TO> o, int v_tiles, int vec) {
+    using S = Shape<L>;
+    extern __shared__ float4 smem4[];
+    const int warps = blockDim.x / 32, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int tile = warps * S::kColumns;
+    float *ks = reinterpret_cast<float *>(smem4), *qs = ks + kBlock * S::kKeyRow, *vs = qs + kBlock * S::kKeyRow, *gs = vs + kBlock * tile;
+    int64_t id = blockIdx.x;
+    const int vt = id % v_tiles;
+    id /= v_tiles;
+    const int seg = id % p.nseg;
+    id /= p.nseg;
+    const int64_t h = id % p.H, b = id / p.H, len = p.length(b);
+    const int l = lane % L, group = lane / L;
+    const int key0 = l * kLaneK, col0 = vt * tile + warp * S::kColumns + group * kLaneV;
+
+    Two state[kLaneV][kLaneK / 2];
+    const float *from = nullptr;
+    int64_t sk = p.Dv, sv = 1;
+    if (p.nseg > 1) {
+        if (kOut) from = p.seg_state + ((b * p.H + h) * p.nseg + seg) * (int64_t)p.Dk * p.Dv;
+    } else if (p.state_in) {
+        from = p.state_in + (b * p.H + h) * (int64_t)p.Dk * p.Dv;
+        sk = p.sk;
+        sv = p.sv;
+    }
+#pragma unroll
+    for (int c = 0; c < kLaneV; ++c)
+#pragma unroll
+        for (int i = 0; i < kLaneK / 2; ++i) {
+            float e[2] = {0.f, 0.f};
+            if (from && col0 + c < p.Dv) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+                    if (key0 + 2 * i + j < p.Dk) e[j] = from[(key0 + 2 * i + j) * sk + (col0 + c) * sv];
+            }
+            state[c][i] = two(e[0], e[1]);
+        }
+
+    const int64_t begin = seg * p.seg_len, end = min((int64_t)p.T, begin + p.seg_len);
+    double total = 0.0;      // threads of the first warp: their share of the logarithm of the segment's decay
+    for (int64_t s0 = begin; s0 < min(end, len); s0 += kBlock) {
+        const int rows = (int)min((int64_t)kBlock, min(end, len) - s0);
+        __syncthreads();
+        stage<T, true>(ks, S::kKeyRow, k, p, b, h, s0, rows, len, 0, p.Dk, L * kLaneK, 1.f, vec);
+        if (kOut) stage<T, true>(qs, S::kKeyRow, q, p, b, h, s0, rows, len, 0, p.Dk, L * kLaneK, 1.f, vec);
+        stage<T, false>(vs, tile, v, p, b, h, s0, rows, len, vt * tile, p.Dv - vt * tile, tile, p.in_scale, vec);
+        if (threadIdx.x < rows) {      // (kBlock is a warp)
+            const float e = p.log_decay(b, h, s0 + threadIdx.x, len);
+            const double a = exp((double)e);
+            gs[2 * threadIdx.x] = (float)a;
+            gs[2 * threadIdx.x + 1] = (float)(a - (float)a);
+            total += e;
+        }
+        __syncthreads();
+        for (int r = 0; r < rows; ++r) {
+            const Two decay = splat(gs[2 * r]), fine = splat(gs[2 * r + 1]);
+            const float4 v4 = *reinterpret_cast<const float4 *>(vs + r * tile + warp * S::kColumns + group * kLaneV);
+            const Two vv[4] = {splat(v4.x), splat(v4.y), splat(v4.z), splat(v4.w)};
+            Two acc[4] = {splat(0.f), splat(0.f), splat(0.f), splat(0.f)};
+            const float4 *kr = reinterpret_cast<const float4 *>(ks + r * S::kKeyRow + l * kPitch);
+            const float4 *qr = reinterpret_cast<const float4 *>(qs + r * S::kKeyRow + l * kPitch);
+#pragma unroll
+            for (int i = 0; i < kLaneK / 4; ++i) {
+                const float4 k4 = kr[i];
+                const Two k0 = two(k4.x, k4.y), k1 = two(k4.z, k4.w);
+                Two q0, q1;
+                if (kOut) {
+                    const float4 q4 = qr[i];
+                    q0 = two(q4.x, q4.y);
+                    q1 = two(q4.z, q4.w);
+                }
+#pragma unroll
+                for (int c = 0; c < kLaneV; ++c) {
+                    state[c][2 * i] = fma2(decay, state[c][2 * i], fma2(fine, state[c][2 * i], mul2(k0, vv[c])));
+                    state[c][2 * i + 1] = fma2(decay, state[c][2 * i + 1], fma2(fine, state[c][2 * i + 1], mul2(k1, vv[c])));
+                    if (kOut) {
+                        acc[c] = fma2(q0, state[c][2 * i], acc[c]);
+                        acc[c] = fma2(q1, state[c][2 * i + 1], acc[c]);
+                    }
+                }
+            }
+            if (kOut) {
+                float sum[4];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    float x, y;
+                    split(acc[c], x, y);
+                    sum[c] = x + y;
+                }
+                // the lanes of a group share the sums out: each step halves the channels that a lane still adds up
+                int kept = 4, first = 0;
+                if (L >= 2) {
+                    constexpr int m = L / 2;
+                    const bool up = l & m;
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        const float mine = up ? sum[c + 2] : sum[c], other = up ? sum[c] : sum[c + 2];
+                        sum[c] = mine + __shfl_xor_sync(0xffffffffu, other, m);
+                    }
+                    kept = 2;
+                    first = up ? 2 : 0;
+                }
+                if (L >= 4) {
+                    constexpr int m = L / 4 > 0 ? L / 4 : 1;
+                    const bool up = l & m;
+                    const float mine = up ? sum[1] : sum[0], other = up ? sum[0] : sum[1];
+                    sum[0] = mine + __shfl_xor_sync(0xffffffffu, other, m);
+                    kept = 1;
+                    first += up ? 1 : 0;
+                }
+                if (L >= 8) {
+                    sum[0] += __shfl_xor_sync(0xffffffffu, sum[0], 1);
+                    kept = l & 1 ? 0 : 1;
+                }
+                TO *row = o.row(b, p.token(s0 + r, len), h);
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    if (c < kept && col0 + first + c < p.Dv) row[col0 + first + c] = (TO)(sum[c] * p.out_scale);
+            }
+        }
+    }
+    if (kOut) {
+        const int64_t z0 = max(begin, len), columns = min(tile, p.Dv - vt * tile);
+        for (int64_t i = threadIdx.x; i < (end - z0) * columns; i += blockDim.x) o.row(b, z0 + i / columns, h)[vt * tile + i % columns] = (TO)0.f;
+        if (p.nseg > 1 || !p.state_out) return;
+    }
+    float *to;
+    float last = 1.f;
+    if (kOut) {
+        to = p.state_out + (b * p.H + h) * (int64_t)p.Dk * p.Dv;
+        sk = p.sk;
+        sv = p.sv;
+        if (p.reverse && len > 0) last = expf(p.g[b * p.gsb + h * p.gsh]);
+    } else {
+        to = p.seg_state + ((b * p.H + h) * p.nseg + seg) * (int64_t)p.Dk * p.Dv;
+        sk = p.Dv;
+        sv = 1;
+        for (int w = 16; w; w >>= 1) total += __shfl_xor_sync(0xffffffffu, total, w);
+        if (threadIdx.x == 0 && vt == 0) p.seg_decay[(b * p.H + h) * p.nseg + seg] = (float)exp(total);
+    }
+#pragma unroll
+    for (int c = 0; c < kLaneV; ++c)
+#pragma unroll
+        for (int i = 0; i < kLaneK / 2; ++i) {
+            float e[2];
+            split(state[c][i], e[0], e[1]);
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+                if (key0 + 2 * i + j < p.Dk && col0 + c < p.Dv) to[(key0 + 2 * i + j) * sk + (col0 + c) * sv] = e[j] * last;
+        }
+}
+
+// The segments' own sums, in order, into the states that enter them: in place, one thread for each state element.
+__global__ void __launch_bounds__(256) fold_segments(Problem p) {
+    const int64_t n = (int64_t)p.Dk * p.Dv, per = (n + blockDim.x - 1) / blockDim.x;
+    const int64_t bh = blockIdx.x / per, i = blockIdx.x % per * blockDim.x + threadIdx.x;
+    if (i >= n) return;
+    const int64_t at = bh * n + i / p.Dv * p.sk + i % p.Dv * p.sv;
+    float *seg = p.seg_state + bh * p.nseg * n + i;
+    const float *decay = p.seg_decay + bh * p.nseg;
+    float s = p.state_in ? p.state_in[at] : 0.f;
+    for (int j = 0; j < p.nseg; ++j) {
+        const float own = seg[j * n];
+        seg[j * n] = s;
+        s = fmaf(decay[j], s, own);
+    }
+    if (p.state_out) {
+        const int64_t b = bh / p.H, h = bh % p.H;
+        p.state_out[at] = p.reverse && p.length(b) > 0 ? s * expf(p.g[b * p.gsb + h * p.gsh]) : s;
+    }
+}
+
+// ------------------------------------------------------------------ one token
+// S <- e^g S + k v^T and o = q^T S with the state in place: nothing but a pass over the states, 8 bytes an element.
+// A CTA takes kStepColumns-wide columns of one state; its threads hold V neighbouring value channels and every
+// (threads / lanes)-th key channel, so a row is read in full sectors and kStepBatch rows are in flight for each thread.
+constexpr int kStepThreads = 128, kStepBatch = 8;
+
+template <typename T, int V>
+__global__ void __launch_bounds__(kStepThreads) step(int64_t B, int64_t H, int Dk, int Dv, Heads<const T> q, Heads<const T> k, Heads<const T> v, Heads<T> o,
+                                                     const float *g, int64_t gsb, int64_t gsh, float scale, float *states, int64_t ssb, int64_t pool,
+                                                     const int32_t *slots, int tiles, int columns) {
+    __shared__ float ks[kMaxDim], qs[kMaxDim];
+    __shared__ float4 parts[kStepThreads];
+    const int64_t id = blockIdx.x / tiles, b = id / H, h = id % H;
+    const int col0 = blockIdx.x % tiles * columns;
+    const int lanes = columns / V;                    // of a row
+    const int lane = threadIdx.x % lanes, first = threadIdx.x / lanes, rows = kStepThreads / lanes;
+    const int col = col0 + lane * V;
+    const int64_t slot = slots ? slots[b] : b;
+    const bool live = slot >= 0 && slot < pool;      // others (padding of a batch): zeros, and no state is touched
+    T *out = o.row(b, 0, h);
+    if (!live) {
+        for (int i = threadIdx.x; i < columns && col0 + i < Dv; i += kStepThreads) out[col0 + i] = (T)0.f;
+        return;
+    }
+    float *S = states + slot * ssb + h * (int64_t)Dk * Dv;
+    const bool inside = first < rows && col < Dv;
+    float4 held[kStepBatch];
+    const auto load = [&](int r, float4 &x) {
+        if (V == 4) x = *reinterpret_cast<const float4 *>(S + (int64_t)r * Dv + col);
+        else x.x = S[(int64_t)r * Dv + col];
+    };
+    // the first rows travel while the token is fetched
+#pragma unroll
+    for (int j = 0; j < kStepBatch; ++j)
+        if (inside && first + j * rows < Dk) load(first + j * rows, held[j]);
+    const T *kr = k.row(b, 0, h), *qr = q.row(b, 0, h), *vr = v.row(b, 0, h);
+    for (int i = threadIdx.x; i < Dk; i += kStepThreads) {
+        ks[i] = (float)kr[i];
+        qs[i] = (float)qr[i];
+    }
+    float vv[V], acc[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        vv[j] = inside ? (float)vr[col + j] : 0.f;
+        acc[j] = 0.f;
+    }
+    const float decay = expf(g[b * gsb + h * gsh]);
+    __syncthreads();
+    for (int r0 = first; r0 < Dk; r0 += kStepBatch * rows) {
+        if (r0 != first) {
+#pragma unroll
+            for (int j = 0; j < kStepBatch; ++j)
+                if (inside && r0 + j * rows < Dk) load(r0 + j * rows, held[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < kStepBatch; ++j) {
+            const int r = r0 + j * rows;
+            if (!inside || r >= Dk) continue;
+            float x[4] = {held[j].x, held[j].y, held[j].z, held[j].w};
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                x[i] = fmaf(decay, x[i], ks[r] * vv[i]);
+                acc[i] = fmaf(qs[r], x[i], acc[i]);
+            }
+            if (V == 4) *reinterpret_cast<float4 *>(S + (int64_t)r * Dv + col) = make_float4(x[0], x[1], x[2], x[3]);
+            else S[(int64_t)r * Dv + col] = x[0];
+        }
+    }
+    float4 mine = make_float4(acc[0], V == 4 ? acc[V == 4 ? 1 : 0] : 0.f, V == 4 ? acc[V == 4 ? 2 : 0] : 0.f, V == 4 ? acc[V == 4 ? 3 : 0] : 0.f);
+    parts[threadIdx.x] = mine;
+    __syncthreads();
+    if (first == 0 && col < Dv) {
+        for (int r = 1; r < rows; ++r) {
+            const float4 x = parts[r * lanes + lane];
+            mine.x += x.x; mine.y += x.y; mine.z += x.z; mine.w += x.w;
+        }
+        const float x[4] = {mine.x, mine.y, mine.z, mine.w};
+#pragma unroll
+        for (int i = 0; i < V; ++i) out[col + i] = (T)(x[i] * scale);
+    }
+}
+
+// ------------------------------------------------------------------ gradients of shared heads, and of the decays
+// From the gradient of each state's own copy of a tensor, in fp32: the sum over the heads that share it, rounded once,
+// and the dot product of each copy with the tensor itself (what the decays' gradients are made of).  A warp for each
+// row of the tensor.
+template <typename T>
+__global__ void __launch_bounds__(256) finish_gradient(int64_t B, int64_t Tn, int64_t H, int64_t heads, int D, const float *each, Heads<const T> x, Heads<T> dx,
+                                                       float *dots) {
+    const int64_t row = (int64_t)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
+    const int lane = threadIdx.x % 32;
+    if (row >= B * Tn * heads) return;
+    const int64_t hx = row % heads, bt = row / heads, b = bt / Tn, t = bt % Tn, group = H / heads;
+    const float *from = each + (bt * H + hx * group) * D;
+    const T *xr = x.row(b, t, hx * group);
+    T *out = dx.row(b, t, hx * group);
+    float total[kMaxDim / 32];
+#pragma unroll
+    for (int c = 0; c < kMaxDim / 32; ++c) total[c] = 0.f;
+    for (int64_t m = 0; m < group; ++m) {
+        float dot = 0.f;
+#pragma unroll
+        for (int c = 0; c < kMaxDim / 32; ++c) {
+            const int d = c * 32 + lane;
+            if (d < D) {
+                const float e = from[m * D + d];
+                total[c] += e;
+                // (a row beyond the sequence's length has zeros for its gradient, and anything for itself)
+                if (dots && e != 0.f) dot = fmaf(e, (float)xr[d], dot);
+            }
+        }
+        if (dots) {
+            for (int w = 16; w; w >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, w);
+            if (lane == 0) dots[bt * H + hx * group + m] = dot;
+        }
+    }
+#pragma unroll
+    for (int c = 0; c < kMaxDim / 32; ++c)
+        if (c * 32 + lane < D) out[c * 32 + lane] = (T)total[c];
+}
+
+// dL/dg_t = F_t = F_{t+1} + q_t.dq_t - k_t.dk_t, from F = <last state, its gradient> behind the last token; 0 where the
+// decay is 0.  One CTA for each (sequence, head) walks the tokens from the last to the first, 256 at a time; sums in
+// fp64, because F is what large terms of both signs leave.
+// per_token: writes F [B, T, H]; else the sums over the tokens, [B, H].
+constexpr int kFlowThreads = 256;
+__global__ void __launch_bounds__(kFlowThreads) decay_gradient(Problem p, const float *q_dq, const float *k_dk, const float *last, const float *grad_last,
+                                                               float *per_token, float *sums) {
+    __shared__ double part[kFlowThreads / 32], value[kFlowThreads / 32];
+    __shared__ int cut[kFlowThreads / 32];
+    const int64_t b = blockIdx.x / p.H, h = blockIdx.x % p.H, len = p.length(b), n = (int64_t)p.Dk * p.Dv;
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    double flow = 0.0;
+    if (grad_last) {
+        for (int64_t i = threadIdx.x; i < n; i += kFlowThreads) flow += (double)last[(b * p.H + h) * n + i] * grad_last[(b * p.H + h) * n + i];
+        for (int w = 16; w; w >>= 1) flow += __shfl_xor_sync(0xffffffffu, flow, w);
+        if (lane == 0) part[warp] = flow;
+        __syncthreads();
+        flow = 0.0;
+        for (int w = 0; w < kFlowThreads / 32; ++w) flow += part[w];
+    }
+    double sum = 0.0;
+    if (per_token)
+        for (int64_t t = len + threadIdx.x; t < p.T; t += kFlowThreads) per_token[(b * p.T + t) * p.H + h] = 0.f;
+    for (int64_t s0 = 0; s0 < len; s0 += kFlowThreads) {
+        const int64_t s = s0 + threadIdx.x, t = len - 1 - s;
+        double x = 0.0;
+        bool zero = false;      // what came before this visit no longer counts behind it
+        if (s < len) {
+            const int64_t at = (b * p.T + t) * p.H + h;
+            x = (double)q_dq[at] - (double)k_dk[at];
+            if (expf(p.g[b * p.gsb + t * p.gst + h * p.gsh]) == 0.f) { x = 0.0; zero = true; }
+        }
+        for (int w = 1; w < 32; w <<= 1) {
+            const double px = __shfl_up_sync(0xffffffffu, x, w);
+            const bool pz = __shfl_up_sync(0xffffffffu, (int)zero, w);
+            if (lane >= w) {
+                if (!zero) x += px;
+                zero |= pz;
+            }
+        }
+        __syncthreads();
+        if (lane == 31) { value[warp] = x; cut[warp] = zero; }
+        __syncthreads();
+        double enter = flow;
+        for (int w = 0; w < kFlowThreads / 32; ++w) {
+            if (w == warp) enter = flow;
+            flow = cut[w] ? value[w] : flow + value[w];
+        }
+        if (!zero) x += enter;
+        if (s < len) {
+            if (per_token) per_token[(b * p.T + t) * p.H + h] = (float)x;
+            sum += x;
+        }
+    }
+    if (sums) {
+        for (int w = 16; w; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+        __syncthreads();
+        if (lane == 0) part[warp] = sum;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            sum = 0.0;
+            for (int w = 0; w < kFlowThreads / 32; ++w) sum += part[w];
+            sums[b * p.H + h] = (float)sum;
+        }
+    }
+}
+
+// The gradient of decays that all sequences and tokens share: the sums over the sequences, in order.
+__global__ void __launch_bounds__(128) sum_sequences(int64_t B, int64_t H, const float *sums, float *out) {
+    const int64_t h = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    if (h >= H) return;
+    double s = 0.0;
+    for (int64_t b = 0; b < B; ++b) s += sums[b * H + h];
+    out[h] = (float)s;
+}
+
+// ------------------------------------------------------------------ host side
+constexpr int kPlannedSms = 148;      // segment lengths are planned for this many multiprocessors on every device, so that results do not depend on it
+
+// How many segments a sequence is cut into: `units` CTAs take one segment each, `slots` of them run at a time.  The
+// segments' own sums cost `extra` of a pass, and folding them about `fold` tokens' time for each segment; the shortest
+// total wins.  A segment is a multiple of `block` tokens.
+inline int choose_segments(int64_t units, int64_t T, int64_t slots, int64_t block, double extra, double fold) {
+    const int64_t blocks = T > 0 ? ceil_div(T, block) : 1;
+    int best = 1;
+    double least = 0.0;
+    for (int n = 1; n <= 128 && n <= blocks; ++n) {
+        const int64_t per = ceil_div(blocks, n);
+        if (n > 1 && ceil_div(blocks, per) != n) continue;      // (the same segments as a smaller n)
+        const double cost = (double)ceil_div(units * n, slots) * (double)(per * block) * (n > 1 ? 1.0 + extra : 1.0) + (n > 1 ? fold * n : 0.0);
+        if (n == 1 || cost < least) { least = cost; best = n; }
+    }
+    return best;
+}
+
+}  // namespace linattn
+}  // namespace fss

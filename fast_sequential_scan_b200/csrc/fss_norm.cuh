@@ -1,0 +1,379 @@
+// Root-mean-square norm of the sum of a tensor and the residual stream:
+//
+//     s = round(x + residual) ,   r = 1 / sqrt(mean(s^2) + eps) ,   y = s r w
+//
+// s is what the stream keeps (in the tensors' type), and what is normalised, so that the backward needs s and nothing
+// else; sums and r are fp32.  Outputs of 8 bits (e4m3) hold y / scale with scale = max|y| / 448 over a row or a group of
+// channels.
+//     dx = dresidual = r (w dy) - s r^3 mean(s w dy) + ds ,    dw = sum over the rows of dy s r
+//
+// Bound by memory: x, residual, s, y once each; backward dy, ds, s, dx.  A row's elements stay in registers between the
+// sum and the output.
+#pragma once
+
+#include <cuda_fp8.h>
+
+#include "fss_common.cuh"
+
+namespace fss {
+namespace norm {
+
+constexpr float kLargest = 448.f;      // of e4m3
+constexpr float kLeast = 1e-30f;       // rows with no larger value than this are held as zeros times their scale
+
+enum Quant { kNone = 0, kRow = 1, kGroup = 2 };
+
+template <typename T> struct Params {
+    int64_t B, T_, D;
+    View<const T> x, residual;      // residual.ptr NULL: none
+    View<T> sum;                    // s, written where there is a residual
+    View<T> y;
+    __nv_fp8_e4m3 *held;            // [B, T, D], contiguous
+    float *scales;                  // [B, T] or [B, T, D / group]
+    float *rstd;                    // [B, T] or NULL
+    const void *weight;
+    float eps;
+    int group;
+};
+
+template <int V> __device__ __forceinline__ void load_weight(const void *w, bool wide, int64_t at, float (&f)[V]) {
+    if (wide) {
+        const float *p = static_cast<const float *>(w) + at;
+        if (V % 4 == 0) {
+#pragma unroll
+            for (int i = 0; i < V; i += 4) {
+                const float4 x = __ldg(reinterpret_cast<const float4 *>(p + i));
+                f[i] = x.x; f[(i + 1) % V] = x.y; f[(i + 2) % V] = x.z; f[(i + 3) % V] = x.w;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) f[i] = p[i];
+        }
+    } else {
+        const bf16 *p = static_cast<const bf16 *>(w) + at;
+        if (V % 8 == 0) {
+            const uint4 x = __ldg(reinterpret_cast<const uint4 *>(p));
+            const uint32_t u[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+            for (int i = 0; i < V; ++i) f[i] = __uint_as_float(i % 2 ? u[i / 2 % 4] & 0xffff0000u : u[i / 2 % 4] << 16);
+        } else if (V % 4 == 0) {
+            const uint2 x = __ldg(reinterpret_cast<const uint2 *>(p));
+            const uint32_t u[2] = {x.x, x.y};
+#pragma unroll
+            for (int i = 0; i < V; ++i) f[i] = __uint_as_float(i % 2 ? u[i / 2 % 2] & 0xffff0000u : u[i / 2 % 2] << 16);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) f[i] = __bfloat162float(p[i]);
+        }
+    }
+}
+
+// what a stored value of type T is worth
+template <typename T> __device__ __forceinline__ float stored(float x);
+template <> __device__ __forceinline__ float stored<bf16>(float x) { return __bfloat162float(__float2bfloat16_rn(x)); }
+template <> __device__ __forceinline__ float stored<float>(float x) { return x; }
+
+// the largest magnitude, a NaN where there is one
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+template <int V> __device__ __forceinline__ void store_held(__nv_fp8_e4m3 *p, const float (&f)[V], float inverse) {
+    uint8_t b[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) b[i] = __nv_cvt_float_to_fp8(f[i] * inverse, __NV_SATFINITE, __NV_E4M3);
+    if (V == 8) {
+        uint2 u;
+        memcpy(&u, b, 8);
+        *reinterpret_cast<uint2 *>(p) = u;
+    } else if (V == 4) {
+        uint32_t u;
+        memcpy(&u, b, 4);
+        *reinterpret_cast<uint32_t *>(p) = u;
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) reinterpret_cast<uint8_t *>(p)[i] = b[i];
+    }
+}
+
+// ------------------------------------------------------------------ sums over the threads of a row
+// `threads`: of a row, a warp (several rows a CTA) or the CTA.  Every thread gets the result.
+struct Sum { static __device__ __forceinline__ float of(float a, float b) { return a + b; } };
+struct Most { static __device__ __forceinline__ float of(float a, float b) { return max_nan(a, b); } };
+
+template <bool kBlockRow, typename Op> __device__ __forceinline__ float over_row(float x, float *shared) {
+#pragma unroll
+    for (int w = 16; w; w >>= 1) x = Op::of(x, __shfl_xor_sync(0xffffffffu, x, w));
+    if (!kBlockRow) return x;
+    const int warps = blockDim.x / 32;
+    if (warps == 1) return x;
+    __syncthreads();      // (the values of the sum before are read)
+    if (threadIdx.x % 32 == 0) shared[threadIdx.x / 32] = x;
+    __syncthreads();
+    x = shared[0];
+    for (int w = 1; w < warps; ++w) x = Op::of(x, shared[w]);
+    return x;
+}
+
+// ------------------------------------------------------------------ forward, rows in registers
+// N fragments of V channels a thread.  kBlockRow: a CTA for each row; else a warp.
+template <typename T, int N, bool kBlockRow, int kQuant>
+__global__ void __launch_bounds__(kBlockRow ? 1024 : 256) forward(Params<T> p, bool wide) {
+    constexpr int V = VecWidth<T>::value;
+    __shared__ float shared[32];
+    const int threads = kBlockRow ? blockDim.x : 32, me = kBlockRow ? threadIdx.x : threadIdx.x % 32;
+    const int64_t row = kBlockRow ? blockIdx.x : (int64_t)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
+    if (row >= p.B * p.T_) return;      // (whole warps)
+    const int64_t b = row / p.T_, t = row % p.T_;
+    const int n = (int)(p.D / V);
+    const T *x = p.x.row(b, t), *res = p.residual.ptr ? p.residual.row(b, t) : nullptr;
+    typename Frag<T, V>::Raw raw[N], more[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const int at = me + j * threads;
+        if (at < n) {
+            raw[j] = Frag<T, V>::load_raw(x + (int64_t)at * V);
+            if (res) more[j] = Frag<T, V>::load_raw(res + (int64_t)at * V);
+        }
+    }
+    float f[N][V], sum = 0.f;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const int at = me + j * threads;
+        if (at < n) {
+            Frag<T, V>::unpack(raw[j], f[j]);
+            if (res) {
+                float g[V];
+                Frag<T, V>::unpack(more[j], g);
+#pragma unroll
+                for (int i = 0; i < V; ++i) f[j][i] = stored<T>(f[j][i] + g[i]);
+                Frag<T, V>::store(p.sum.row(b, t) + (int64_t)at * V, f[j]);
+            }
+#pragma unroll
+            for (int i = 0; i < V; ++i) sum = fmaf(f[j][i], f[j][i], sum);
+        }
+    }
+    sum = over_row<kBlockRow, Sum>(sum, shared);
+    const float r = rsqrtf(sum / (float)p.D + p.eps);
+    if (p.rstd && me == 0) p.rstd[row] = r;
+    float most = 0.f;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const int at = me + j * threads;
+        if (at < n) {
+            float w[V];
+            load_weight<V>(p.weight, wide, (int64_t)at * V, w);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                f[j][i] = f[j][i] * r * w[i];
+                if (kQuant == kRow) most = max_nan(most, fabsf(f[j][i]));
+            }
+            if (kQuant == kNone) Frag<T, V>::store(p.y.row(b, t) + (int64_t)at * V, f[j]);
+        }
+    }
+    if (kQuant == kRow) {
+        most = over_row<kBlockRow, Most>(most, shared);
+        if (me == 0) p.scales[row] = most / kLargest;
+        const float inverse = kLargest / max_nan(most, kLeast);
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int at = me + j * threads;
+            if (at < n) store_held<V>(p.held + row * p.D + (int64_t)at * V, f[j], inverse);
+        }
+    }
+    if (kQuant == kGroup) {
+        // neighbouring lanes hold neighbouring fragments: a group is an aligned run of group / V lanes (at most a warp)
+        const int run = p.group / V;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int at = me + j * threads;
+            float m = 0.f;
+            if (at < n) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) m = max_nan(m, fabsf(f[j][i]));
+            }
+            for (int w = run / 2; w; w >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, w));
+            if (at < n) {
+                if (at % run == 0) p.scales[row * (n / run) + at / run] = m / kLargest;
+                store_held<V>(p.held + row * p.D + (int64_t)at * V, f[j], kLargest / max_nan(m, kLeast));
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------ forward, any width, alignment and type
+// A CTA for each row, one channel at a time; the row is read again for the output.
+template <typename T, int kQuant> __global__ void __launch_bounds__(256) forward_any(Params<T> p, bool wide) {
+    __shared__ float shared[32];
+    const int64_t row = blockIdx.x, b = row / p.T_, t = row % p.T_;
+    const T *x = p.x.row(b, t), *res = p.residual.ptr ? p.residual.row(b, t) : nullptr;
+    const T *kept = res ? p.sum.row(b, t) : x;      // (a thread reads back what it wrote itself)
+    const auto value = [&](int64_t d) { return (float)kept[d]; };
+    const auto weight = [&](int64_t d) {
+        float w[1];
+        load_weight<1>(p.weight, wide, d, w);
+        return w[0];
+    };
+    float sum = 0.f;
+    for (int64_t d = threadIdx.x; d < p.D; d += blockDim.x) {
+        if (res) p.sum.row(b, t)[d] = (T)((float)x[d] + (float)res[d]);
+        const float f = value(d);
+        sum = fmaf(f, f, sum);
+    }
+    sum = over_row<true, Sum>(sum, shared);
+    const float r = rsqrtf(sum / (float)p.D + p.eps);
+    if (p.rstd && threadIdx.x == 0) p.rstd[row] = r;
+    if (kQuant == kNone) {
+        for (int64_t d = threadIdx.x; d < p.D; d += blockDim.x) p.y.row(b, t)[d] = (T)(value(d) * r * weight(d));
+        return;
+    }
+    // one group after the other: the whole row, or runs of p.group channels
+    const int64_t run = kQuant == kRow ? p.D : p.group, groups = p.D / run;
+    for (int64_t g = 0; g < groups; ++g) {
+        float most = 0.f;
+        for (int64_t d = g * run + threadIdx.x; d < (g + 1) * run; d += blockDim.x) most = max_nan(most, fabsf(value(d) * r * weight(d)));
+        most = over_row<true, Most>(most, shared);
+        if (threadIdx.x == 0) p.scales[row * groups + g] = most / kLargest;
+        const float inverse = kLargest / max_nan(most, kLeast);
+        for (int64_t d = g * run + threadIdx.x; d < (g + 1) * run; d += blockDim.x) {
+            const float f[1] = {value(d) * r * weight(d)};
+            store_held<1>(p.held + row * p.D + d, f, inverse);
+        }
+    }
+}
+
+// ------------------------------------------------------------------ backward
+// CTAs walk the rows with the grid's stride and keep the weight's gradient of their rows in registers; `parts`
+// [parts, D] gets one row of sums from each, which sum_parts adds up in order (the same bits in every run on one
+// device).
+template <typename T> struct BackwardParams {
+    int64_t B, T_, D;
+    View<const T> s, dy, dsum;      // dsum.ptr NULL: no gradient arrives for the sum
+    View<T> dx;
+    const float *rstd;
+    const void *weight;
+    float *parts;                   // NULL: the weight's gradient is not wanted
+};
+
+template <typename T, int N, bool kBlockRow>
+__global__ void __launch_bounds__(kBlockRow ? 1024 : 256) backward(BackwardParams<T> p, bool wide) {
+    constexpr int V = VecWidth<T>::value;
+    __shared__ float shared[32];
+    const int threads = kBlockRow ? blockDim.x : 32, me = kBlockRow ? threadIdx.x : threadIdx.x % 32;
+    const int64_t walkers = kBlockRow ? gridDim.x : (int64_t)gridDim.x * (blockDim.x / 32);
+    const int64_t walker = kBlockRow ? blockIdx.x : (int64_t)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
+    const int n = (int)(p.D / V);
+    float dw[N][V];
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+#pragma unroll
+        for (int i = 0; i < V; ++i) dw[j][i] = 0.f;
+    for (int64_t row = walker; row < p.B * p.T_; row += walkers) {
+        const int64_t b = row / p.T_, t = row % p.T_;
+        typename Frag<T, V>::Raw rs[N], rg[N], ra[N];
+        const float r = p.rstd[row];
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int at = me + j * threads;
+            if (at < n) {
+                rs[j] = Frag<T, V>::load_raw(p.s.row(b, t) + (int64_t)at * V);
+                rg[j] = Frag<T, V>::load_raw(p.dy.row(b, t) + (int64_t)at * V);
+                if (p.dsum.ptr) ra[j] = Frag<T, V>::load_raw(p.dsum.row(b, t) + (int64_t)at * V);
+            }
+        }
+        float dot = 0.f;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int at = me + j * threads;
+            if (at < n) {
+                float s[V], g[V], w[V];
+                Frag<T, V>::unpack(rs[j], s);
+                Frag<T, V>::unpack(rg[j], g);
+                load_weight<V>(p.weight, wide, (int64_t)at * V, w);
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    dw[j][i] = fmaf(g[i], s[i] * r, dw[j][i]);
+                    dot = fmaf(g[i] * w[i], s[i], dot);
+                }
+            }
+        }
+        dot = over_row<kBlockRow, Sum>(dot, shared);
+        const float c = dot / (float)p.D * r * r * r;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int at = me + j * threads;
+            if (at < n) {
+                float s[V], g[V], w[V];
+                Frag<T, V>::unpack(rs[j], s);
+                Frag<T, V>::unpack(rg[j], g);
+                load_weight<V>(p.weight, wide, (int64_t)at * V, w);
+#pragma unroll
+                for (int i = 0; i < V; ++i) g[i] = fmaf(g[i] * w[i], r, -s[i] * c);
+                if (p.dsum.ptr) {
+                    float a[V];
+                    Frag<T, V>::unpack(ra[j], a);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) g[i] += a[i];
+                }
+                Frag<T, V>::store(p.dx.row(b, t) + (int64_t)at * V, g);
+            }
+        }
+    }
+    if (!p.parts) return;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const int at = me + j * threads;
+        if (at < n)
+#pragma unroll
+            for (int i = 0; i < V; ++i) p.parts[walker * p.D + (int64_t)at * V + i] = dw[j][i];
+    }
+}
+
+// Any width and alignment: CTA c takes the rows c, c + parts, ...; its sums go to its own row of `parts` in memory.
+template <typename T> __global__ void __launch_bounds__(256) backward_any(BackwardParams<T> p, bool wide) {
+    __shared__ float shared[32];
+    const auto weight = [&](int64_t d) {
+        float w[1];
+        load_weight<1>(p.weight, wide, d, w);
+        return w[0];
+    };
+    float *part = p.parts ? p.parts + blockIdx.x * p.D : nullptr;
+    if (part)
+        for (int64_t d = threadIdx.x; d < p.D; d += blockDim.x) part[d] = 0.f;      // (each thread only ever touches its own channels)
+    for (int64_t row = blockIdx.x; row < p.B * p.T_; row += gridDim.x) {
+        const int64_t b = row / p.T_, t = row % p.T_;
+        const T *s = p.s.row(b, t), *dy = p.dy.row(b, t), *dsum = p.dsum.ptr ? p.dsum.row(b, t) : nullptr;
+        const float r = p.rstd[row];
+        float dot = 0.f;
+        for (int64_t d = threadIdx.x; d < p.D; d += blockDim.x) {
+            dot = fmaf((float)dy[d] * weight(d), (float)s[d], dot);
+            if (part) part[d] = fmaf((float)dy[d], (float)s[d] * r, part[d]);
+        }
+        dot = over_row<true, Sum>(dot, shared);
+        const float c = dot / (float)p.D * r * r * r;
+        for (int64_t d = threadIdx.x; d < p.D; d += blockDim.x)
+            p.dx.row(b, t)[d] = (T)(fmaf((float)dy[d] * weight(d), r, -(float)s[d] * c) + (dsum ? (float)dsum[d] : 0.f));
+    }
+}
+
+// dw[d] = sum over the parts, in order: 8 warps take every eighth part of 32 channels, then their sums are added.
+__global__ void __launch_bounds__(256) sum_parts(const float *parts, int64_t count, int64_t D, void *dw, bool wide) {
+    __shared__ float share[8][32];
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    const int64_t d = (int64_t)blockIdx.x * 32 + lane;
+    float s = 0.f;
+    if (d < D)
+        for (int64_t i = warp; i < count; i += 8) s += parts[i * D + d];
+    share[warp][lane] = s;
+    __syncthreads();
+    if (warp == 0 && d < D) {
+        for (int w = 1; w < 8; ++w) s += share[w][lane];
+        if (wide) static_cast<float *>(dw)[d] = s;
+        else static_cast<bf16 *>(dw)[d] = __float2bfloat16_rn(s);
+    }
+}
+
+}  // namespace norm
+}  // namespace fss

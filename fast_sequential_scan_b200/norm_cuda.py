@@ -1,0 +1,135 @@
+"""Root-mean-square norm with the residual stream's addition, and with an output of 8 bits.
+
+    s = x + residual   (rounded to the tensors' type: what the stream keeps, and what is normalised)
+    y = s * weight / sqrt(mean(s^2) + eps)
+
+:func:`rms_norm` returns ``y`` (and ``s``) and is differentiable.  :func:`rms_norm_quantized` holds ``y`` as
+``torch.float8_e4m3fn`` with a scale for each row or each group of channels (``y = held * scale``, the largest value of a
+row or group at 448), for the 8-bit product that follows; it is for serving and has no gradient.
+
+The norm is over the last dimension; any leading dimensions.  ``weight``: a vector of the tensors' type or fp32.  Sums are
+fp32, ``y`` is rounded once.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional
+
+import torch
+from torch.autograd import Function
+from torch.autograd.function import once_differentiable
+
+from . import _lib, workspace
+from .attention_cuda import _DTYPES, _check, _pointer
+from .sequential_scan_cuda import _rowwise, _view
+
+GROUPS = (32, 64, 128)
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """``[batch, seq, channels]`` that the kernels can address, without a copy where there is one."""
+    return _rowwise(t if t.dim() == 3 else t.reshape(1, -1, t.shape[-1]))
+
+
+def _check_inputs(x, weight, residual):
+    _check("x", x, x.dim() if isinstance(x, torch.Tensor) else 1, None)
+    if x.dtype not in _DTYPES:
+        raise RuntimeError(f"x: unsupported dtype {x.dtype} (bf16 or fp32)")
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise RuntimeError(f"x: expected channels in the last dimension, got {tuple(x.shape)}")
+    _check("weight", weight, 1, x)
+    if weight.dtype not in (x.dtype, torch.float32):
+        raise RuntimeError(f"weight: expected dtype {x.dtype} or torch.float32, got {weight.dtype}")
+    if weight.shape[0] != x.shape[-1]:
+        raise RuntimeError(f"weight: {weight.shape[0]} values for {x.shape[-1]} channels")
+    if residual is not None:
+        _check("residual", residual, x.dim(), x, x.dtype)
+        if residual.shape != x.shape:
+            raise RuntimeError(f"residual: shape {tuple(residual.shape)} differs from {tuple(x.shape)}")
+
+
+def _forward(x, weight, residual, eps: float, want_rstd: bool, quantized: bool = False, group: Optional[int] = None):
+    """``(y or held, s or None, rstd or None, scales or None)``"""
+    new = lambda dtype, *shape: torch.empty(shape, dtype=dtype, device=x.device)
+    D = x.shape[-1]
+    out = new(torch.float8_e4m3fn if quantized else x.dtype, *x.shape)
+    s = new(x.dtype, *x.shape) if residual is not None else None
+    rstd = new(torch.float32, *x.shape[:-1]) if want_rstd else None
+    scales = new(torch.float32, *x.shape[:-1], *([D // group] if group else [])) if quantized else None
+    if x.numel():
+        weight = weight.contiguous()
+        rows = [_rows(t) if t is not None else None for t in (x, residual, s)]
+        views = [_view(t) if t is not None else None for t in rows]
+        refs = [ctypes.byref(v) if v is not None else None for v in views]
+        w = _lib.NormWeight(weight.data_ptr(), _DTYPES[weight.dtype])
+        o = _lib.NormOutput(_lib.View() if quantized else _view(_rows(out)), out.data_ptr() if quantized else None, _pointer(scales), _pointer(rstd),
+                            group or 0)
+        ctx = workspace.call_context(x.device)
+        _lib.check(_lib.lib().fss_rms_norm_forward(ctypes.byref(ctx), _DTYPES[x.dtype], *rows[0].shape, refs[0], refs[1], ctypes.byref(w), eps, refs[2],
+                                                   ctypes.byref(o)), "fss_rms_norm_forward")
+    return out, s, rstd, scales
+
+
+def _backward(s, weight, rstd, dy, dsum, want_weight: bool):
+    dx = torch.empty(s.shape, dtype=s.dtype, device=s.device)
+    dw = torch.empty(weight.shape, dtype=weight.dtype, device=s.device) if want_weight else None
+    if s.numel() == 0:
+        return dx, dw.zero_() if dw is not None else None
+    weight = weight.contiguous()
+    rows = [_rows(t) if t is not None else None for t in (s, dy, dsum, dx)]
+    views = [_view(t) if t is not None else None for t in rows]
+    refs = [ctypes.byref(v) if v is not None else None for v in views]
+    scratch = None
+    if want_weight:
+        scratch = torch.empty(_lib.lib().fss_rms_norm_workspace_bytes(s.shape[-1]), dtype=torch.uint8, device=s.device)
+    ctx = workspace.call_context(s.device, scratch)
+    w = _lib.NormWeight(weight.data_ptr(), _DTYPES[weight.dtype])
+    _lib.check(_lib.lib().fss_rms_norm_backward(ctypes.byref(ctx), _DTYPES[s.dtype], *rows[0].shape, refs[0], ctypes.byref(w), rstd.data_ptr(), refs[1],
+                                                refs[2], refs[3], _pointer(dw)), "fss_rms_norm_backward")
+    return dx, dw
+
+
+class RmsNorm(Function):
+    """Inputs: x, weight, residual (or None), eps.  Outputs: y, and s with a residual."""
+
+    @staticmethod
+    def forward(ctx, x, weight, residual, eps):
+        y, s, rstd, _ = _forward(x, weight, residual, eps, True)
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(s if residual is not None else x, weight, rstd)
+        return (y, s) if residual is not None else y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dsum=None):
+        s, weight, rstd = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        if dy is None:
+            dy = torch.zeros(s.shape, dtype=s.dtype, device=s.device)
+        dx, dw = _backward(s, weight, rstd, dy.to(s.dtype), dsum.to(s.dtype) if dsum is not None else None, need[1])
+        return dx if need[0] else None, dw, dx if need[2] else None, None
+
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor, *, residual: Optional[torch.Tensor] = None, eps: float = 1e-6):
+    """``y``, or ``(y, s)`` with a ``residual``; see the module's docstring.  Differentiable with respect to ``x``,
+    ``weight`` and ``residual``."""
+    _check_inputs(x, weight, residual)
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad)):
+        return RmsNorm.apply(x, weight, residual, float(eps))
+    y, s, _, _ = _forward(x, weight, residual, float(eps), False)
+    return (y, s) if residual is not None else y
+
+
+def rms_norm_quantized(x: torch.Tensor, weight: torch.Tensor, *, residual: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                       group: Optional[int] = None):
+    """``(held, scales)``, or ``(held, scales, s)`` with a ``residual``.  ``held``: ``torch.float8_e4m3fn`` of x's shape;
+    ``scales``: fp32, one a row (``x.shape[:-1]``), or with ``group`` (32, 64 or 128, a divisor of the channels) one for
+    each group of channels (``[..., channels // group]``).  A row or group whose largest value is below 1e-30 keeps its
+    zeros and loses what is smaller.  Not differentiable."""
+    _check_inputs(x, weight, residual)
+    if group is not None and (group not in GROUPS or x.shape[-1] % group):
+        raise ValueError(f"group={group}: expected one of {GROUPS} that divides {x.shape[-1]} channels")
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad)):
+        raise RuntimeError("rms_norm_quantized is not differentiable: use rms_norm, or torch.no_grad()")
+    held, s, _, scales = _forward(x, weight, residual, float(eps), False, True, group)
+    return (held, scales, s) if residual is not None else (held, scales)

@@ -1,0 +1,137 @@
+"""Rotary positions for queries and keys.
+
+The first ``rotary_dim`` channels of every head are pairs ``(x, y)`` -- channels ``(2j, 2j+1)`` in the ``"interleaved"``
+layout, ``(j, j + rotary_dim/2)`` in the ``"half"`` layout -- and the pair ``j`` of a token at position ``p`` is turned by
+``p * turns[j]`` full turns; the other channels pass through.
+
+``turns`` is a vector of 64-bit fractions of a full turn (``round(frequency / (2 pi) * 2**64)``, as int64), made once by
+:func:`rotary_turns`.  The product with an integer position, modulo 2**64, is then the exact fraction of a turn: angles are
+as good at position 10,000,000 as at position 1, and no table of sines limits the length.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import Any, Mapping, Optional, Tuple
+
+import torch
+from torch.autograd import Function
+from torch.autograd.function import once_differentiable
+
+from . import _lib, workspace
+from .attention_cuda import _DTYPES, _channels, _check, _heads
+
+LAYOUTS = ("half", "interleaved")
+MAX_ROTARY_DIM = 1024
+
+
+def rotary_turns(rotary_dim: int, *, base: float = 10000.0, scaling: Optional[Mapping[str, Any]] = None, device=None
+                 ) -> Tuple[torch.Tensor, float]:
+    """``(turns, magnitude)`` for :func:`rotary`: pair ``j`` turns by ``base ** (-2j / rotary_dim)`` radians a position.
+
+    ``scaling`` stretches the positions for contexts ``factor`` times longer than those of training:
+
+    ``{"type": "linear", "factor": f}``      every angle divided by ``f``
+    ``{"type": "base", "factor": f}``        a larger base: the slowest pair is divided by ``f``, the fastest kept
+    ``{"type": "parts", "factor": f, "length": n}``  pairs that make more than ``fast`` (32) turns in ``n`` positions are
+        kept, those that make fewer than ``slow`` (1) are divided by ``f``, a linear ramp over the pairs' indices between
+        them; queries and keys grow by ``magnitude`` (``0.1 ln f + 1`` unless given)
+    """
+    if rotary_dim < 2 or rotary_dim % 2 or rotary_dim > MAX_ROTARY_DIM:
+        raise ValueError(f"rotary_dim={rotary_dim}: expected an even number from 2 to {MAX_ROTARY_DIM}")
+    if not base > 0:
+        raise ValueError(f"base={base}: expected a positive number")
+    pairs = rotary_dim // 2
+    magnitude = 1.0
+    stretch = [1.0] * pairs
+    if scaling is not None:
+        kind, factor = scaling.get("type"), float(scaling.get("factor", 0.0))
+        if kind not in ("linear", "base", "parts") or not factor > 0:
+            raise ValueError(f"scaling={dict(scaling)}: expected a type of 'linear', 'base' or 'parts' and a positive factor")
+        if kind == "linear":
+            stretch = [factor] * pairs
+        elif kind == "base":
+            if rotary_dim > 2:
+                base = base * factor ** (rotary_dim / (rotary_dim - 2))
+        else:
+            length, fast, slow = float(scaling["length"]), float(scaling.get("fast", 32.0)), float(scaling.get("slow", 1.0))
+            index = lambda rounds: rotary_dim * math.log(length / (rounds * 2 * math.pi)) / (2 * math.log(base))
+            low, high = max(math.floor(index(fast)), 0), min(math.ceil(index(slow)), rotary_dim - 1)
+            for j in range(pairs):
+                kept = 1.0 - min(1.0, max(0.0, (j - low) / max(high - low, 1e-3)))
+                stretch[j] = 1.0 / (kept + (1.0 - kept) / factor)
+            magnitude = float(scaling.get("magnitude", 0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0))
+    words = []
+    for j in range(pairs):
+        word = round(base ** (-2.0 * j / rotary_dim) / stretch[j] / (2 * math.pi) * 2.0**64) % 2**64
+        words.append(word - 2**64 if word >= 2**63 else word)
+    return torch.tensor(words, dtype=torch.int64, device=device), magnitude
+
+
+def _apply(q, k, positions, turns, layout: str, magnitude: float, inverse: bool):
+    q = _channels(q)
+    outs = [torch.empty(q.shape, dtype=q.dtype, device=q.device)]
+    sides = [_heads(q), None]
+    if k is not None:
+        k = _channels(k)
+        outs.append(torch.empty(k.shape, dtype=k.dtype, device=k.device))
+        sides[1] = _heads(k)
+    sb, st = (0, positions.stride(0)) if positions.dim() == 1 else positions.stride()
+    r = _lib.Rotary(ctypes.sizeof(_lib.Rotary), int(layout == "interleaved"), int(inverse), magnitude, 2 * turns.numel(), positions.data_ptr(), sb, st,
+                    turns.data_ptr())
+    ctx = workspace.call_context(q.device)
+    _lib.check(_lib.lib().fss_rotary_apply(ctypes.byref(ctx), _DTYPES[q.dtype], q.shape[0], q.shape[1], ctypes.byref(sides[0]),
+                                           ctypes.byref(sides[1]) if k is not None else None, outs[0].data_ptr(),
+                                           outs[1].data_ptr() if k is not None else None, ctypes.byref(r)), "fss_rotary_apply")
+    return outs
+
+
+class Rotary(Function):
+    """Inputs: q, k (or None), positions, turns, layout, magnitude.  The gradient is the opposite rotation."""
+
+    @staticmethod
+    def forward(ctx, q, k, positions, turns, layout, magnitude):
+        outs = _apply(q, k, positions, turns, layout, magnitude, False)
+        ctx.save_for_backward(positions, turns)
+        ctx.layout, ctx.magnitude = layout, magnitude
+        return tuple(outs) if k is not None else outs[0]
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_q, grad_k=None):
+        positions, turns = ctx.saved_tensors
+        outs = _apply(grad_q, grad_k, positions, turns, ctx.layout, ctx.magnitude, True)
+        return outs[0], outs[1] if grad_k is not None else None, None, None, None, None
+
+
+def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, turns: torch.Tensor, *, layout: str = "half",
+           magnitude: float = 1.0):
+    """``(q', k')`` with the positions turned in; ``q'`` alone when ``k`` is None.  Differentiable with respect to q and k.
+
+    ``q``, ``k``: ``[batch, seq, heads, dim]``, bf16 or fp32, any strides with neighbouring channels.  ``positions``: integers
+    ``[seq]`` or ``[batch, seq]``, any values.  ``turns``, ``magnitude``: from :func:`rotary_turns`; ``2 * turns.numel()``
+    channels of each head are turned."""
+    _check("q", q, 4, None)
+    if q.dtype not in _DTYPES:
+        raise RuntimeError(f"q: unsupported dtype {q.dtype} (bf16 or fp32)")
+    if k is not None:
+        _check("k", k, 4, q, q.dtype)
+        if k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3]:
+            raise RuntimeError(f"k: shape {tuple(k.shape)} does not go with {tuple(q.shape)}")
+    _check("turns", turns, 1, q, torch.int64)
+    if not 1 <= turns.numel() <= MAX_ROTARY_DIM // 2 or 2 * turns.numel() > q.shape[3]:
+        raise RuntimeError(f"turns: {turns.numel()} pairs for heads of {q.shape[3]} channels (at most {MAX_ROTARY_DIM // 2} are supported)")
+    if layout not in LAYOUTS:
+        raise ValueError(f"layout must be one of {LAYOUTS}, got {layout!r}")
+    if not isinstance(positions, torch.Tensor) or positions.is_floating_point() or positions.is_complex() or positions.dtype == torch.bool:
+        raise TypeError("positions must be a tensor of integers")
+    _check("positions", positions, positions.dim(), q)
+    if positions.shape != q.shape[1:2] and positions.shape != q.shape[:2]:
+        raise RuntimeError(f"positions: expected [{q.shape[1]}] or [{q.shape[0]}, {q.shape[1]}], got {list(positions.shape)}")
+    if q.shape[2] < 1 or (k is not None and k.shape[2] < 1):
+        raise RuntimeError("q, k: no heads")
+    positions, turns = positions.to(torch.int64), turns.contiguous()
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        return Rotary.apply(q, k, positions, turns, layout, float(magnitude))
+    outs = _apply(q, k, positions, turns, layout, float(magnitude), False)
+    return tuple(outs) if k is not None else outs[0]

@@ -28,6 +28,7 @@ it, and a workspace is never replaced by a larger one between the look-up and th
 """
 from __future__ import annotations
 
+import ctypes
 import threading
 
 import torch
@@ -158,6 +159,24 @@ def get_locked(device: torch.device, nbytes: int) -> Workspace:
     if ws.order.last is not ws:
         ws.order_after_other_streams()
     return ws
+
+
+def call_context(device: torch.device, scratch=None) -> _lib.ScanCtx:
+    """What the library is handed for a launch that waits for no other CTA: the current stream, its status word and the
+    call's own scratch (a tensor, or None).  Such launches are not ordered against those of other streams."""
+    index = device.index if device.index is not None else torch.cuda.current_device()
+    stream = current_stream_handle(device)
+    ws = _cache.get((index, stream))
+    if ws is None:
+        with _lock:
+            ws = _cache.get((index, stream))
+            if ws is None:
+                ws = _cache[(index, stream)] = Workspace(torch.device("cuda", index), stream)
+    if ws._flag[0]:
+        with ws.order.lock:
+            ws.raise_if_flagged()
+    return _lib.ScanCtx(ctypes.sizeof(_lib.ScanCtx), index, stream, scratch.data_ptr() if scratch is not None else None,
+                        scratch.numel() if scratch is not None else 0, ws.status.data_ptr(), _lib.ALGO_AUTO, 0)
 
 
 def launched(ws: Workspace) -> None:

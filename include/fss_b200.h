@@ -375,6 +375,101 @@ int fss_seqpar_fixup_backward_from(const fss_scan_ctx *ctx, int dtype, int64_t B
                                    const fss_carry_source *source, const float *h_prev, const float *block_prod,
                                    const float *block_state, int64_t block_rows);
 
+/* ---- operators of layers with a matrix state -------------------------------------------------
+ * No counterparts in the reference.  They take an fss_scan_ctx like the scans do; `algo`, `flags` and the
+ * look-back launches' ordering play no part (no kernel here waits for another CTA), and `workspace` is plain
+ * scratch of the call: at least the bytes that the matching query names, 16-byte aligned, uninitialised,
+ * free again when the launches have run (NULL where the query says 0). */
+
+/* One [B, T, heads, dim] tensor: element (b, t, h, d) lives at ptr + (b*stride_b + t*stride_t + h*stride_h + d)
+ * elements.  Input strides may be 0 (broadcast); an output's elements must not share memory. */
+typedef struct fss_heads {
+    void *ptr;
+    int64_t stride_b, stride_t, stride_h;
+    int64_t heads, dim;
+} fss_heads;
+
+/* Linear attention with a decay for each head.  For every sequence and head a state S [Dk, Dv] in fp32,
+ *     S_t = exp(log_decay_t) S_{t-1} + k_t v_t^T ;   o_t = scale * q_t^T S_t ,
+ * from S_{-1} = h0.  A log decay of -inf empties the state before token t is added.
+ * q [B, T, Hq, Dk], k [B, T, Hk, Dk], v [B, T, Hv, Dv]: Hq, Hk, Hv each divide H, and head h reads head
+ * h / (H / Hq) of q and so on.  Dk, Dv <= 256 (FSS_E_TOO_LARGE), T < 2^31. */
+typedef struct fss_linear_attention {
+    uint32_t struct_bytes; /* sizeof(fss_linear_attention) */
+    int32_t dtype;         /* FSS_DTYPE_*, of q, k, v, o and their gradients */
+    int64_t B, T, H;
+    fss_heads q, k, v;
+    const float *log_decay; /* fp32, element (b, t, h) at b*stride_b + t*stride_t + h*stride_h; strides of 0
+                               for what does not depend on the sequence or the token */
+    int64_t decay_stride_b, decay_stride_t, decay_stride_h;
+    const int32_t *lengths; /* [B] on the device: tokens of each sequence that count (clamped to 0 .. T); the
+                               rows behind them are not read, their outputs and gradients are zeros.  NULL: T */
+    const float *h0;        /* [B, H, Dk, Dv] fp32, contiguous; NULL: zeros */
+    float scale;
+} fss_linear_attention;
+
+/* backward: 0 the forward, 1 the gradients, 2 the gradients with those of the decays */
+size_t fss_linear_attention_workspace_bytes(const fss_linear_attention *p, int backward);
+/* o [B, T, H, Dv]; h_last [B, H, Dk, Dv] or NULL: the state behind the last token. */
+int fss_linear_attention_forward(const fss_scan_ctx *ctx, const fss_linear_attention *p, const fss_heads *o, float *h_last);
+/* Gradients from those of o and (grad_last, NULL: none) of h_last.  dq, dk, dv have the heads of q, k, v: the heads
+ * of a group are summed in fp32 and rounded once; each may be NULL, but grad_decay needs dq and dk and grad_h0 needs
+ * dv (FSS_E_NULL).  grad_decay (or NULL): [B, T, H] with per_token, else [H].  h_last: what the forward returned,
+ * needed for grad_decay with grad_last. */
+int fss_linear_attention_backward(const fss_scan_ctx *ctx, const fss_linear_attention *p, const fss_heads *grad_o,
+                                  const float *h_last, const float *grad_last, const fss_heads *dq, const fss_heads *dk,
+                                  const fss_heads *dv, float *grad_decay, int per_token, float *grad_h0);
+/* One token for each sequence (T = 1, no lengths, no h0), the state in place: sequence b has its state at
+ * states + slot * state_stride, slot = slots[b], or b without slots.  A slot outside 0 .. pool-1 marks a row of
+ * padding: zeros, and no state is touched.  Two sequences of a call must not share a slot. */
+int fss_linear_attention_step(const fss_scan_ctx *ctx, const fss_linear_attention *p, const fss_heads *o, float *states,
+                              int64_t state_stride, int64_t pool, const int32_t *slots);
+
+/* Root-mean-square norm over the D channels of each row, of s = round(x + residual) to `dtype` (s = x without a
+ * residual):  y = s * r * weight,  r = 1 / sqrt(mean(s^2) + eps).  Sums and r in fp32. */
+typedef struct fss_norm_weight {
+    const void *ptr; /* [D] */
+    int32_t dtype;   /* the tensors' type or FSS_DTYPE_F32 */
+} fss_norm_weight;
+/* One of y and held: y [B, T, D] of `dtype`, or held [B, T, D] contiguous bytes of e4m3 with y = held * scale,
+ * scale = max|y| / 448 over the row (scales [B, T], group 0) or over each `group` = 32, 64 or 128 channels
+ * (scales [B, T, D / group]).  Where max|y| is below 1e-30, held is y * (448 / 1e-30).  rstd [B, T] or NULL: r, for
+ * the backward. */
+typedef struct fss_norm_output {
+    fss_view y;
+    void *held;
+    float *scales;
+    float *rstd;
+    int32_t group;
+} fss_norm_output;
+/* sum: where s goes; needed with a residual, unused without; overlaps neither. */
+int fss_rms_norm_forward(const fss_scan_ctx *ctx, int dtype, int64_t B, int64_t T, int64_t D, const fss_view *x,
+                         const fss_view *residual, const fss_norm_weight *weight, float eps, const fss_view *sum,
+                         const fss_norm_output *out);
+/* dx = r (w dy) - s r^3 mean(s w dy) + dsum (the gradient of x and of the residual), dweight [D] of the weight's type,
+ * or NULL; dsum: the gradient that arrives for s, or NULL.  The workspace is used for dweight. */
+size_t fss_rms_norm_workspace_bytes(int64_t D);
+int fss_rms_norm_backward(const fss_scan_ctx *ctx, int dtype, int64_t B, int64_t T, int64_t D, const fss_view *s,
+                          const fss_norm_weight *weight, const float *rstd, const fss_view *dy, const fss_view *dsum,
+                          const fss_view *dx, void *dweight);
+
+/* Rotary positions: the first rotary_dim channels of every head of q and k as pairs (x, y), channels (2j, 2j+1) when
+ * interleaved, else (j, j + rotary_dim/2); pair j of a token at position p is turned by p * turns[j] turns,
+ *     x' = magnitude * (x cos - y sin) ,  y' = magnitude * (x sin + y cos) ;
+ * with `inverse` by the opposite angle.  turns[j] / 2^64 of a full turn, so that p * turns[j] mod 2^64 is exact for any
+ * position.  q_out, k_out: contiguous [B, T, heads, dim].  k may be NULL.  rotary_dim <= 1024. */
+typedef struct fss_rotary {
+    uint32_t struct_bytes; /* sizeof(fss_rotary) */
+    int32_t interleaved, inverse;
+    float magnitude;
+    int64_t rotary_dim;
+    const int64_t *positions; /* of (b, t): positions[b*position_stride_b + t*position_stride_t] */
+    int64_t position_stride_b, position_stride_t;
+    const int64_t *turns; /* [rotary_dim / 2] */
+} fss_rotary;
+int fss_rotary_apply(const fss_scan_ctx *ctx, int dtype, int64_t B, int64_t T, const fss_heads *q, const fss_heads *k,
+                     void *q_out, void *k_out, const fss_rotary *rotary);
+
 #ifdef __cplusplus
 }
 #endif
