@@ -1,6 +1,11 @@
 // Host side of the C entry points, shared by the library's translation units: errors, the current device, checks.
 #pragma once
 
+#include <cuda.h>
+
+#include <mutex>
+#include <string>
+
 #include "fss_common.cuh"
 
 #define FSS_API extern "C" __attribute__((visibility("default")))
@@ -59,6 +64,25 @@ inline int multiprocessors() {
         cached[dev] = (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess && n > 0) ? n : 148;
     }
     return cached[dev];
+}
+
+// the driver's encoder of TMA descriptors, looked up once; NULL where there is none
+typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                                  const cuuint64_t *, const cuuint32_t *, const cuuint32_t *,
+                                  CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
+                                  CUtensorMapFloatOOBfill);
+
+inline EncodeTiledFn encode_fn() {
+    static EncodeTiledFn fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void *ptr = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<EncodeTiledFn>(ptr);
+    });
+    return fn;
 }
 
 }  // namespace fss

@@ -1,6 +1,7 @@
 // C entry points of linear attention (include/fss_b200.h): argument checks, plans, launches.
 #include "fss_host.cuh"
 #include "fss_linattn.cuh"
+#include "fss_linattn_mma.cuh"
 
 namespace fss {
 namespace linattn {
@@ -43,22 +44,35 @@ static int check_problem(const fss_linear_attention *p) {
 }
 
 // ------------------------------------------------------------------ plans
+// One pass over tensors of key dimension Dk and value dimension Dv: on the tensor cores for key dimensions up to 128,
+// else by the recurrent kernels.
 struct Plan {
-    int lanes, warps, v_tiles, nseg;
+    bool matrix;
+    int lanes, warps;      // recurrent kernels
+    int v_tiles, nseg;
     int64_t seg_len;
     size_t seg_bytes;      // states and decays of the segments
 };
 
-// One pass over tensors of key dimension Dk and value dimension Dv.
-static Plan make_plan(int64_t B, int64_t T, int64_t H, int64_t Dk, int64_t Dv) {
+static Plan make_plan(int64_t B, int64_t T, int64_t H, int64_t Dk, int64_t Dv, bool fine) {
     Plan w{};
-    w.lanes = Dk <= 32 ? 1 : Dk <= 64 ? 2 : Dk <= 128 ? 4 : 8;
-    const int64_t columns = 32 / w.lanes * kLaneV;
-    w.warps = (int)(ceil_div(Dv, columns) < 4 ? ceil_div(Dv, columns) : 4);
-    w.v_tiles = (int)ceil_div(Dv, columns * w.warps);
-    // two CTAs of four warps a multiprocessor (registers); a pass for the sums alone does two thirds of the work
-    w.nseg = choose_segments(B * H * w.v_tiles, T, kPlannedSms * (8 / w.warps), kBlock, 0.67, 4.0);
-    w.seg_len = ceil_div(ceil_div(T > 0 ? T : 1, kBlock), w.nseg) * kBlock;
+    w.matrix = Dk <= 128 && T > kShort;
+    int64_t block;
+    if (w.matrix) {
+        block = mma::kChunk;
+        w.v_tiles = (int)ceil_div(Dv, mma::kValues);
+        // one CTA a multiprocessor with three pieces of everything, else two
+        w.nseg = choose_segments(B * H * w.v_tiles, T, kPlannedSms * (fine ? 1 : 2), block, {0.5, 128.0, 256.0, 0.7});
+    } else {
+        block = kBlock;
+        w.lanes = Dk <= 32 ? 1 : Dk <= 64 ? 2 : Dk <= 128 ? 4 : 8;
+        const int64_t columns = 32 / w.lanes * kLaneV;
+        w.warps = (int)(ceil_div(Dv, columns) < 4 ? ceil_div(Dv, columns) : 4);
+        w.v_tiles = (int)ceil_div(Dv, columns * w.warps);
+        // two CTAs of four warps a multiprocessor (registers); a pass for the sums alone does two thirds of the work
+        w.nseg = choose_segments(B * H * w.v_tiles, T, kPlannedSms * (8 / w.warps), block, {0.67, 8.0, 16.0, 0.1});
+    }
+    w.seg_len = ceil_div(ceil_div(T > 0 ? T : 1, block), w.nseg) * block;
     w.seg_bytes = w.nseg > 1 ? align_up((size_t)(B * H * w.nseg) * (size_t)(Dk * Dv + 1) * sizeof(float), 256) : 0;
     return w;
 }
@@ -116,9 +130,72 @@ template <typename T, typename TO, int L> static int run_recurrent(const Problem
     return launch_check("linear attention launch");
 }
 
-template <typename T, typename TO> static int run_pass(const fss_linear_attention *p, const Pass &s, const fss_heads *o, void *scratch, cudaStream_t stream) {
-    const Plan w = make_plan(p->B, p->T, p->H, s.q.dim, s.v.dim);
+// A 4-d map of a tensor of 16-bit values, with boxes of 64 channels x 64 tokens; false where TMA cannot address it.
+static bool make_map(CUtensorMap *map, const fss_heads &x, int64_t B, int64_t T) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn || !aligned16(x.ptr)) return false;
+    const int64_t extent[4] = {x.dim, x.heads, T, B}, stride[4] = {1, x.stride_h, x.stride_t, x.stride_b};
+    cuuint64_t dims[4], strides[3];
+    for (int i = 0; i < 4; ++i) {
+        if (extent[i] > UINT32_MAX) return false;
+        dims[i] = (cuuint64_t)extent[i];
+        if (i == 0) continue;
+        // (the stride of a single element is never used)
+        const int64_t bytes = extent[i] > 1 ? stride[i] * 2 : (x.dim + 7) / 8 * 16;
+        if (bytes <= 0 || bytes % 16 || bytes >= 1ll << 40) return false;
+        strides[i - 1] = (cuuint64_t)bytes;
+    }
+    const cuuint32_t box[4] = {64, 1, (cuuint32_t)mma::kChunk, 1}, step[4] = {1, 1, 1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, x.ptr, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, typename TO, int KD, int kLoad, int kInput, int kState>
+static int run_chunked(const Problem &x, const Plan &w, const Pass &s, const fss_heads *o, const mma::Maps &maps, int flags, int32_t *status, cudaStream_t stream) {
+    const auto q = make_heads<const T>(&s.q, x.H), k = make_heads<const T>(&s.k, x.H), v = make_heads<const T>(&s.v, x.H);
+    const auto out = make_heads<TO>(o, x.H);
+    const int64_t blocks = x.B * x.H * w.nseg * w.v_tiles;
+    if (blocks > INT32_MAX) return FSS_E_SHAPE;
+    constexpr int few = mma::Plan<KD, kInput, kState, false>::kShared, all = mma::Plan<KD, kInput, kState, true>::kShared;
+    auto *sums = mma::chunked<T, TO, KD, kLoad, kInput, kState, false>;
+    auto *outputs = mma::chunked<T, TO, KD, kLoad, kInput, kState, true>;
+    FSS_CUDA(cudaFuncSetAttribute(outputs, cudaFuncAttributeMaxDynamicSharedMemorySize, all), "shared memory of a chunked pass");
+    if (w.nseg > 1) {
+        FSS_CUDA(cudaFuncSetAttribute(sums, cudaFuncAttributeMaxDynamicSharedMemorySize, few), "shared memory of a chunked pass");
+        sums<<<(unsigned)blocks, mma::kThreads, few, stream>>>(x, maps, q, k, v, out, w.v_tiles, flags, status);
+        fold_segments<<<(unsigned)(x.B * x.H * ceil_div((int64_t)x.Dk * x.Dv, 256)), 256, 0, stream>>>(x);
+    }
+    outputs<<<(unsigned)blocks, mma::kThreads, all, stream>>>(x, maps, q, k, v, out, w.v_tiles, flags, status);
+    return launch_check("linear attention launch");
+}
+
+// fine: outputs in all 24 bits (they are fp32, or the decays' gradients are made of them)
+template <typename T, typename TO> static int run_pass(const fss_linear_attention *p, const Pass &s, const fss_heads *o, bool fine, void *scratch, int32_t *status,
+                                                       cudaStream_t stream) {
+    const Plan w = make_plan(p->B, p->T, p->H, s.q.dim, s.v.dim, fine || sizeof(T) == 4);
     const Problem x = make_problem(p, s, w, scratch);
+    if (w.matrix) {
+        mma::Maps maps{};
+        const auto out = make_heads<TO>(o, x.H);
+        const int vec = wide_rows(make_heads<const T>(&s.q, x.H), x.Dk) && wide_rows(make_heads<const T>(&s.k, x.H), x.Dk) &&
+                        wide_rows(make_heads<const T>(&s.v, x.H), x.Dv);
+        const int packed = x.Dv % 2 == 0 && out.sb % 2 == 0 && out.st % 2 == 0 && out.sh % 2 == 0 && reinterpret_cast<uintptr_t>(out.ptr) % 4 == 0;
+        const int flags = vec | packed << 1;
+        const bool narrow = x.Dk <= 64;
+#define FSS_CHUNKED(LOAD, INPUT, STATE)                                                                                   \
+    (narrow ? run_chunked<T, TO, 64, LOAD, INPUT, STATE>(x, w, s, o, maps, flags, status, stream)                         \
+            : run_chunked<T, TO, 128, LOAD, INPUT, STATE>(x, w, s, o, maps, flags, status, stream))
+        if constexpr (sizeof(T) == 4) {
+            return FSS_CHUNKED(mma::kPlain, 3, 3);
+        } else {
+            const bool tma = make_map(&maps.q, s.q, x.B, x.T) && make_map(&maps.k, s.k, x.B, x.T) && make_map(&maps.v, s.v, x.B, x.T);
+            if constexpr (sizeof(TO) == 4) {
+                if (fine) return tma ? FSS_CHUNKED(mma::kTma, 1, 3) : FSS_CHUNKED(mma::kPlain, 1, 3);
+            }
+            return tma ? FSS_CHUNKED(mma::kTma, 1, 1) : FSS_CHUNKED(mma::kPlain, 1, 1);
+        }
+#undef FSS_CHUNKED
+    }
     if (w.lanes == 1) return run_recurrent<T, TO, 1>(x, w, s, o, stream);
     if (w.lanes == 2) return run_recurrent<T, TO, 2>(x, w, s, o, stream);
     if (w.lanes == 4) return run_recurrent<T, TO, 4>(x, w, s, o, stream);
@@ -133,7 +210,8 @@ struct BackwardPlan {
 static BackwardPlan plan_backward(const fss_linear_attention *p, bool decays) {
     BackwardPlan w{};
     const int64_t n = p->B * p->T * p->H, Dk = p->q.dim, Dv = p->v.dim;
-    const size_t a = make_plan(p->B, p->T, p->H, Dv, Dk).seg_bytes, b = make_plan(p->B, p->T, p->H, Dk, Dv).seg_bytes;
+    const bool f32 = p->dtype == FSS_DTYPE_F32;
+    const size_t a = make_plan(p->B, p->T, p->H, Dv, Dk, decays || f32).seg_bytes, b = make_plan(p->B, p->T, p->H, Dk, Dv, f32).seg_bytes;
     w.seg = a > b ? a : b;
     w.dq_each = decays || p->q.heads < p->H;
     w.dk_each = decays || p->k.heads < p->H;
@@ -148,11 +226,11 @@ static BackwardPlan plan_backward(const fss_linear_attention *p, bool decays) {
 // One of the three gradients: straight to its tensor, or by way of fp32 copies for each state.
 template <typename T>
 static int run_gradient(const fss_linear_attention *p, const Pass &s, const fss_heads &x, const fss_heads *dx, bool by_state, float *each, float *dots,
-                        void *scratch, cudaStream_t stream) {
-    if (!by_state) return run_pass<T, T>(p, s, dx, scratch, stream);
+                        void *scratch, int32_t *status, cudaStream_t stream) {
+    if (!by_state) return run_pass<T, T>(p, s, dx, false, scratch, status, stream);
     const int64_t D = s.v.dim;
     const fss_heads o{each, p->T * p->H * D, p->H * D, D, p->H, D};
-    const int rc = run_pass<T, float>(p, s, &o, scratch, stream);
+    const int rc = run_pass<T, float>(p, s, &o, dots != nullptr, scratch, status, stream);
     if (rc) return rc;
     const int64_t blocks = ceil_div(p->B * p->T * x.heads, 8);
     if (blocks > INT32_MAX) return FSS_E_SHAPE;
@@ -174,15 +252,15 @@ static int run_backward(const fss_scan_ctx *ctx, const fss_linear_attention *p, 
     int rc;
     if (dq || grad_decay) {
         const Pass s{*grad_o, p->v, p->k, 1.f, p->scale, false, true, p->h0, nullptr};
-        if ((rc = run_gradient<T>(p, s, p->q, dq, w.dq_each, each, q_dq, scratch, stream))) return rc;
+        if ((rc = run_gradient<T>(p, s, p->q, dq, w.dq_each, each, q_dq, scratch, ctx->status, stream))) return rc;
     }
     if (dk || grad_decay) {
         const Pass s{p->v, *grad_o, p->q, p->scale, 1.f, true, true, grad_last, nullptr};
-        if ((rc = run_gradient<T>(p, s, p->k, dk, w.dk_each, each, k_dk, scratch, stream))) return rc;
+        if ((rc = run_gradient<T>(p, s, p->k, dk, w.dk_each, each, k_dk, scratch, ctx->status, stream))) return rc;
     }
     if (dv || grad_h0) {
         const Pass s{p->k, p->q, *grad_o, p->scale, 1.f, true, false, grad_last, grad_h0};
-        if ((rc = run_gradient<T>(p, s, p->v, dv, w.dv_each, each, nullptr, scratch, stream))) return rc;
+        if ((rc = run_gradient<T>(p, s, p->v, dv, w.dv_each, each, nullptr, scratch, ctx->status, stream))) return rc;
     }
     if (grad_decay) {
         Problem x{};
@@ -211,7 +289,7 @@ static bool big_enough(const fss_scan_ctx *ctx, size_t need) {
 
 FSS_API size_t fss_linear_attention_workspace_bytes(const fss_linear_attention *p, int backward) {
     if (check_problem(p) || p->B == 0) return 0;
-    if (!backward) return make_plan(p->B, p->T, p->H, p->q.dim, p->v.dim).seg_bytes;
+    if (!backward) return make_plan(p->B, p->T, p->H, p->q.dim, p->v.dim, p->dtype == FSS_DTYPE_F32).seg_bytes;
     const BackwardPlan w = plan_backward(p, backward > 1);
     return w.seg + w.each + 2 * w.dots + w.sums;
 }
@@ -227,8 +305,8 @@ FSS_API int fss_linear_attention_forward(const fss_scan_ctx *ctx, const fss_line
     DeviceGuard guard(ctx->device);
     if (guard.error) return guard.error;
     const Pass s{p->q, p->k, p->v, 1.f, p->scale, false, false, p->h0, h_last};
-    return p->dtype == FSS_DTYPE_BF16 ? run_pass<bf16, bf16>(p, s, o, ctx->workspace, (cudaStream_t)ctx->stream)
-                                      : run_pass<float, float>(p, s, o, ctx->workspace, (cudaStream_t)ctx->stream);
+    return p->dtype == FSS_DTYPE_BF16 ? run_pass<bf16, bf16>(p, s, o, false, ctx->workspace, ctx->status, (cudaStream_t)ctx->stream)
+                                      : run_pass<float, float>(p, s, o, false, ctx->workspace, ctx->status, (cudaStream_t)ctx->stream);
 }
 
 FSS_API int fss_linear_attention_backward(const fss_scan_ctx *ctx, const fss_linear_attention *p, const fss_heads *grad_o, const float *h_last,

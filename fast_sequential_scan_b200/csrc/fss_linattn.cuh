@@ -26,6 +26,7 @@ namespace fss {
 namespace linattn {
 
 constexpr int kMaxDim = 256;      // of keys and values
+constexpr int kShort = 16;        // tokens up to which the recurrent kernels take every call
 
 template <typename T> struct Heads {
     T *ptr;
@@ -276,10 +277,21 @@ __global__ void __launch_bounds__(256) fold_segments(Problem p) {
     float *seg = p.seg_state + bh * p.nseg * n + i;
     const float *decay = p.seg_decay + bh * p.nseg;
     float s = p.state_in ? p.state_in[at] : 0.f;
-    for (int j = 0; j < p.nseg; ++j) {
-        const float own = seg[j * n];
-        seg[j * n] = s;
-        s = fmaf(decay[j], s, own);
+    constexpr int kAhead = 8;      // in flight for each thread
+    for (int j0 = 0; j0 < p.nseg; j0 += kAhead) {
+        float own[kAhead], a[kAhead];
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j)
+            if (j0 + j < p.nseg) {
+                own[j] = seg[(j0 + j) * n];
+                a[j] = decay[j0 + j];
+            }
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j)
+            if (j0 + j < p.nseg) {
+                seg[(j0 + j) * n] = s;
+                s = fmaf(a[j], s, own[j]);
+            }
     }
     if (p.state_out) {
         const int64_t b = bh / p.H, h = bh % p.H;
@@ -487,17 +499,20 @@ __global__ void __launch_bounds__(128) sum_sequences(int64_t B, int64_t H, const
 // ------------------------------------------------------------------ host side
 constexpr int kPlannedSms = 148;      // segment lengths are planned for this many multiprocessors on every device, so that results do not depend on it
 
-// How many segments a sequence is cut into: `units` CTAs take one segment each, `slots` of them run at a time.  The
-// segments' own sums cost `extra` of a pass, and folding them about `fold` tokens' time for each segment; the shortest
-// total wins.  A segment is a multiple of `block` tokens.
-inline int choose_segments(int64_t units, int64_t T, int64_t slots, int64_t block, double extra, double fold) {
+// How many segments a sequence is cut into: `units` CTAs take one segment each, `slots` of them run at a time.  Costs in
+// the time that a CTA takes for a token: the segments' own sums are `extra` of a pass; what a CTA does once (its
+// state, to begin with) is `once`; folding is `launch` and `fold` for each unit's segment.  The shortest total
+// wins.  A segment is a multiple of `block` tokens.
+struct SegmentCosts { double extra, once, launch, fold; };
+inline int choose_segments(int64_t units, int64_t T, int64_t slots, int64_t block, const SegmentCosts &c) {
     const int64_t blocks = T > 0 ? ceil_div(T, block) : 1;
     int best = 1;
     double least = 0.0;
     for (int n = 1; n <= 128 && n <= blocks; ++n) {
         const int64_t per = ceil_div(blocks, n);
         if (n > 1 && ceil_div(blocks, per) != n) continue;      // (the same segments as a smaller n)
-        const double cost = (double)ceil_div(units * n, slots) * (double)(per * block) * (n > 1 ? 1.0 + extra : 1.0) + (n > 1 ? fold * n : 0.0);
+        const double pass = (double)ceil_div(units * n, slots) * ((double)(per * block) + c.once);
+        const double cost = n > 1 ? pass * (1.0 + c.extra) + c.launch + c.fold * (double)(units * n) : pass;
         if (n == 1 || cost < least) { least = cost; best = n; }
     }
     return best;

@@ -40,7 +40,7 @@
 #include <mutex>
 #include <string>
 
-#include "fss_common.cuh"
+#include "fss_host.cuh"
 #include "fss_gates.cuh"
 
 namespace fss {
@@ -1562,24 +1562,6 @@ inline bool layout_ok(int64_t B, int64_t Tn, int64_t D, std::initializer_list<co
         if (B > 1 && (v->stride_b * (int64_t)sizeof(T)) >= (1LL << 40)) return false;
     }
     return true;
-}
-
-typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
-                                  const cuuint64_t *, const cuuint32_t *, const cuuint32_t *,
-                                  CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
-                                  CUtensorMapFloatOOBfill);
-
-inline EncodeTiledFn encode_fn() {
-    static EncodeTiledFn fn = nullptr;
-    static std::once_flag once;
-    std::call_once(once, [] {
-        void *ptr = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            fn = reinterpret_cast<EncodeTiledFn>(ptr);
-    });
-    return fn;
 }
 
 // 3-D map (channels, rows, batch) with a (Dc, tile rows, 1) box; out-of-range elements read as zero

@@ -1,0 +1,129 @@
+// The sm_100a instructions that the matrix kernels are made of: shared-memory barriers with bounded waits, TMA tile
+// loads, tensor memory, tcgen05 matrix products.
+#pragma once
+
+#include <cuda.h>
+
+#include "fss_common.cuh"
+
+namespace fss {
+namespace umma {
+
+__device__ __forceinline__ uint32_t shared_address(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+// ------------------------------------------------------------------ barriers in shared memory
+__device__ __forceinline__ void barrier_init(uint32_t bar, uint32_t count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void barrier_expect(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ bool barrier_try(uint32_t bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return done;
+}
+// Waits for the phase, about two seconds at most.  `gave_up` stays set after a wait that ran out; later waits return at
+// once, so that the kernel comes to its end.
+__device__ __forceinline__ void barrier_wait(uint32_t bar, uint32_t parity, bool &gave_up) {
+    if (barrier_try(bar, parity) || gave_up) return;
+    const long long began = clock64();
+    while (!barrier_try(bar, parity)) {
+        if (clock64() - began > (1ll << 32)) {
+            gave_up = true;
+            return;
+        }
+    }
+}
+
+__device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// ------------------------------------------------------------------ TMA
+// One box of a 4-d map (channels, heads, tokens, sequences) into this CTA's shared memory; x is a multiple of 8 channels
+// of 16 bits.
+__device__ __forceinline__ void tma_load(uint32_t to, const CUtensorMap *map, int x, int head, int token, int sequence, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(to), "l"(map),
+        "r"(bar), "r"(x), "r"(head), "r"(token), "r"(sequence)
+        : "memory");
+}
+
+// ------------------------------------------------------------------ tensor memory
+template <int kColumns> __device__ __forceinline__ void tmem_alloc(uint32_t slot) {      // a whole warp
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "n"(kColumns) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+template <int kColumns> __device__ __forceinline__ void tmem_free(uint32_t base) {       // a whole warp
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "n"(kColumns) : "memory");
+}
+__device__ __forceinline__ void tmem_wait_loads() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_stores() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+// 16 columns of the warp's 32 lanes: thread's own lane, neighbouring columns in neighbouring registers
+__device__ __forceinline__ void tmem_load16(uint32_t at, uint32_t *r) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+                   "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(at));
+}
+__device__ __forceinline__ void tmem_store8(uint32_t at, const uint32_t *r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
+                 "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+}
+
+// ------------------------------------------------------------------ matrix products
+// Operands of 16-bit values in shared memory lie in panels of 64 values (128 bytes) a row, rows behind one another, in
+// the 128-byte swizzle (16-byte units of a row are permuted by the row's number modulo 8); a panel starts on 1,024 bytes.
+// "Along": the 64 values of a row are the product's summed dimension; "across": they are the operand's own rows (of the
+// product), and the panel's rows are summed over.  `panel`: bytes from one panel to the next, for operands "across".
+__device__ __forceinline__ uint64_t operand(uint32_t address, uint32_t panel) {
+    return (uint64_t)((address & 0x3ffff) >> 4) | (uint64_t)(panel >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+__host__ __device__ constexpr uint32_t product(int m, int n, bool a_across, bool b_across) {      // bf16 operands, fp32 sums
+    return 1u << 4 | 1u << 7 | 1u << 10 | (a_across ? 1u << 15 : 0u) | (b_across ? 1u << 16 : 0u) | (uint32_t)(n >> 3) << 17 | (uint32_t)(m >> 4) << 24;
+}
+// one thread; 16 steps of the summed dimension
+__device__ __forceinline__ void multiply(uint32_t d, uint64_t a, uint64_t b, uint32_t what, bool add) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(what), "r"((uint32_t)add)
+        : "memory");
+}
+// A in tensor memory: lane = row, two values of the summed dimension in each column
+__device__ __forceinline__ void multiply_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t what, bool add) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(what), "r"((uint32_t)add)
+        : "memory");
+}
+// the barrier is told when all products that this thread issued have been made
+__device__ __forceinline__ void tell_when_done(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+// two fp32 values as bf16 in one word, x in the low half
+__device__ __forceinline__ uint32_t pack(float x, float y) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(y), "f"(x));
+    return r;
+}
+__device__ __forceinline__ float low(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float high(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+
+}  // namespace umma
+}  // namespace fss
