@@ -87,6 +87,7 @@ struct Pass {
     fss_heads q, k, v;
     float in_scale, out_scale;
     bool reverse, transposed;      // transposed: state_in and state_out hold [Dv, Dk]
+    bool exact_state;              // the state in all 24 bits although none is asked for
     const float *state_in;
     float *state_out;
 };
@@ -150,15 +151,15 @@ static bool make_map(CUtensorMap *map, const fss_heads &x, int64_t B, int64_t T)
               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T, typename TO, int KD, int kLoad, int kInput, int kState>
+template <typename T, typename TO, int KD, int kLoad, int kInput, int kState, int kKeys>
 static int run_chunked(const Problem &x, const Plan &w, const Pass &s, const fss_heads *o, const mma::Maps &maps, int flags, int32_t *status, cudaStream_t stream) {
     const auto q = make_heads<const T>(&s.q, x.H), k = make_heads<const T>(&s.k, x.H), v = make_heads<const T>(&s.v, x.H);
     const auto out = make_heads<TO>(o, x.H);
     const int64_t blocks = x.B * x.H * w.nseg * w.v_tiles;
     if (blocks > INT32_MAX) return FSS_E_SHAPE;
-    constexpr int few = mma::Plan<KD, kInput, kState, false>::kShared, all = mma::Plan<KD, kInput, kState, true>::kShared;
-    auto *sums = mma::chunked<T, TO, KD, kLoad, kInput, kState, false>;
-    auto *outputs = mma::chunked<T, TO, KD, kLoad, kInput, kState, true>;
+    constexpr int few = mma::Plan<KD, kInput, kState, kKeys, false>::kShared, all = mma::Plan<KD, kInput, kState, kKeys, true>::kShared;
+    auto *sums = mma::chunked<T, TO, KD, kLoad, kInput, kState, kKeys, false>;
+    auto *outputs = mma::chunked<T, TO, KD, kLoad, kInput, kState, kKeys, true>;
     FSS_CUDA(cudaFuncSetAttribute(outputs, cudaFuncAttributeMaxDynamicSharedMemorySize, all), "shared memory of a chunked pass");
     if (w.nseg > 1) {
         FSS_CUDA(cudaFuncSetAttribute(sums, cudaFuncAttributeMaxDynamicSharedMemorySize, few), "shared memory of a chunked pass");
@@ -180,19 +181,22 @@ template <typename T, typename TO> static int run_pass(const fss_linear_attentio
         const int vec = wide_rows(make_heads<const T>(&s.q, x.H), x.Dk) && wide_rows(make_heads<const T>(&s.k, x.H), x.Dk) &&
                         wide_rows(make_heads<const T>(&s.v, x.H), x.Dv);
         const int packed = x.Dv % 2 == 0 && out.sb % 2 == 0 && out.st % 2 == 0 && out.sh % 2 == 0 && reinterpret_cast<uintptr_t>(out.ptr) % 4 == 0;
-        const int flags = vec | packed << 1;
+        int flags = vec | packed << 1;
         const bool narrow = x.Dk <= 64;
-#define FSS_CHUNKED(LOAD, INPUT, STATE)                                                                                   \
-    (narrow ? run_chunked<T, TO, 64, LOAD, INPUT, STATE>(x, w, s, o, maps, flags, status, stream)                         \
-            : run_chunked<T, TO, 128, LOAD, INPUT, STATE>(x, w, s, o, maps, flags, status, stream))
+#define FSS_CHUNKED(LOAD, INPUT, STATE, KEYS)                                                                             \
+    (narrow ? run_chunked<T, TO, 64, LOAD, INPUT, STATE, KEYS>(x, w, s, o, maps, flags, status, stream)                   \
+            : run_chunked<T, TO, 128, LOAD, INPUT, STATE, KEYS>(x, w, s, o, maps, flags, status, stream))
         if constexpr (sizeof(T) == 4) {
-            return FSS_CHUNKED(mma::kPlain, 3, 3);
+            return FSS_CHUNKED(mma::kPlain, 3, 3, 3);
         } else {
             const bool tma = make_map(&maps.q, s.q, x.B, x.T) && make_map(&maps.k, s.k, x.B, x.T) && make_map(&maps.v, s.v, x.B, x.T);
             if constexpr (sizeof(TO) == 4) {
-                if (fine) return tma ? FSS_CHUNKED(mma::kTma, 1, 3) : FSS_CHUNKED(mma::kPlain, 1, 3);
+                if (fine) return tma ? FSS_CHUNKED(mma::kTma, 1, 3, 3) : FSS_CHUNKED(mma::kPlain, 1, 3, 3);
+            } else {
+                if (make_map(&maps.o, *o, x.B, x.T)) flags |= 4;
             }
-            return tma ? FSS_CHUNKED(mma::kTma, 1, 1) : FSS_CHUNKED(mma::kPlain, 1, 1);
+            if (!s.exact_state && !x.state_out) return tma ? FSS_CHUNKED(mma::kTma, 1, 1, 2) : FSS_CHUNKED(mma::kPlain, 1, 1, 2);
+            return tma ? FSS_CHUNKED(mma::kTma, 1, 1, 3) : FSS_CHUNKED(mma::kPlain, 1, 1, 3);
         }
 #undef FSS_CHUNKED
     }
@@ -251,15 +255,15 @@ static int run_backward(const fss_scan_ctx *ctx, const fss_linear_attention *p, 
     float *sums = w.dots ? reinterpret_cast<float *>(at + w.seg + w.each + 2 * w.dots) : nullptr;
     int rc;
     if (dq || grad_decay) {
-        const Pass s{*grad_o, p->v, p->k, 1.f, p->scale, false, true, p->h0, nullptr};
+        const Pass s{*grad_o, p->v, p->k, 1.f, p->scale, false, true, false, p->h0, nullptr};
         if ((rc = run_gradient<T>(p, s, p->q, dq, w.dq_each, each, q_dq, scratch, ctx->status, stream))) return rc;
     }
     if (dk || grad_decay) {
-        const Pass s{p->v, *grad_o, p->q, p->scale, 1.f, true, true, grad_last, nullptr};
+        const Pass s{p->v, *grad_o, p->q, p->scale, 1.f, true, true, false, grad_last, nullptr};
         if ((rc = run_gradient<T>(p, s, p->k, dk, w.dk_each, each, k_dk, scratch, ctx->status, stream))) return rc;
     }
     if (dv || grad_h0) {
-        const Pass s{p->k, p->q, *grad_o, p->scale, 1.f, true, false, grad_last, grad_h0};
+        const Pass s{p->k, p->q, *grad_o, p->scale, 1.f, true, false, false, grad_last, grad_h0};
         if ((rc = run_gradient<T>(p, s, p->v, dv, w.dv_each, each, nullptr, scratch, ctx->status, stream))) return rc;
     }
     if (grad_decay) {
@@ -304,7 +308,8 @@ FSS_API int fss_linear_attention_forward(const fss_scan_ctx *ctx, const fss_line
     if (!big_enough(ctx, fss_linear_attention_workspace_bytes(p, 0))) return FSS_E_WORKSPACE;
     DeviceGuard guard(ctx->device);
     if (guard.error) return guard.error;
-    const Pass s{p->q, p->k, p->v, 1.f, p->scale, false, false, p->h0, h_last};
+    // (outputs do not depend on whether the state is asked for, bit for bit)
+    const Pass s{p->q, p->k, p->v, 1.f, p->scale, false, false, true, p->h0, h_last};
     return p->dtype == FSS_DTYPE_BF16 ? run_pass<bf16, bf16>(p, s, o, false, ctx->workspace, ctx->status, (cudaStream_t)ctx->stream)
                                       : run_pass<float, float>(p, s, o, false, ctx->workspace, ctx->status, (cudaStream_t)ctx->stream);
 }

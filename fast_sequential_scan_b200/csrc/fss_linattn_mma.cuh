@@ -14,13 +14,15 @@
 //
 // Precision.  A tensor core takes bf16 operands.  A value is handed over as one bf16 (relative error 2^-9), or as the sum of
 // three, which is all 24 bits of an fp32 value; products of pieces whose orders sum to more than two are below 2^-24 and left
-// out.  K' is always three pieces, because the last state is an fp32 result.  Scores and state take one piece for
-// outputs of bf16: each of the two parts of an output has then been rounded once more than the output itself, which
-// together is about as much as the output's own rounding.  They take three where outputs are fp32 (kState = 3), and
-// so do fp32 inputs (kInput = 3).
+// out.  K' takes three pieces where a state is an fp32 result (kKeys = 3) and two, 2^-18, where it only goes into outputs of
+// bf16.  Scores and state take one piece for outputs of bf16: each of the two parts of an output has then been
+// rounded once more than the output itself, which together is about as much as the output's own rounding.  They
+// take three where outputs are fp32 (kState = 3), and so do fp32 inputs (kInput = 3).
 //
-// All exponents are differences G_i - G_j in base 2 with their whole part kept as an integer, exact to 2^-24 whatever lies
-// between; an empty state (-inf) is a step of -2^20.
+// Decays.  G is summed in base 2 as a whole number and a rest; every factor is made from a difference of two sums.  The scores' factors are products
+// of one for the query and one for the key, about the middle of the chunk or the start of their own half of it, so
+// that neither leaves fp32's range; where a half decays by more than 2^-120 (an empty state, -inf, is a step of -2^20) each
+// score gets its own exponential, with the whole part of G as an integer.
 #pragma once
 
 #include "fss_linattn.cuh"
@@ -36,12 +38,13 @@ constexpr int kValues = 128;                                           // value 
 // kLoad: how the tokens come into shared memory
 enum Load { kTma = 0, kPlain = 1 };
 
-template <int KD, int kInput, int kState, bool kOut> struct Plan {
+template <int KD, int kInput, int kState, int kKeys, bool kOut> struct Plan {
     static constexpr int kPanels = KD / 64;
     static constexpr int kKeyPiece = kPanels * kPanel, kValuePiece = 2 * kPanel;
     // Q first: its product reads 128 rows, of which the upper half lies behind its panels
-    static constexpr int kQ = 0, kK = kQ + (kOut ? kInput * kKeyPiece : 0), kV = kK + 3 * kKeyPiece, kP = kV + kInput * kValuePiece;
-    static constexpr int kEnd = kP + (kOut ? kState * kPanel : 0);
+    static constexpr int kQ = 0, kK = kQ + (kOut ? kInput * kKeyPiece : 0), kV = kK + (kKeys > kInput ? kKeys : kInput) * kKeyPiece, kP = kV + kInput * kValuePiece;
+    static constexpr int kY = kP + (kOut ? kState * kPanel : 0);      // outputs on their way, one piece of bf16
+    static constexpr int kEnd = kY + (kOut && kState == 1 ? kValuePiece : 0);
     static constexpr int kShared = kEnd + 1024;      // (the base is moved up to a multiple of 1,024)
     // tensor memory
     static constexpr int kO1 = 0, kScores = 64, kAdded = kOut ? 128 : 0;
@@ -54,60 +57,93 @@ template <int KD, int kInput, int kState, bool kOut> struct Plan {
     }
 };
 
-struct Maps { CUtensorMap q, k, v; };
+struct Maps { CUtensorMap q, k, v, o; };
 
 // What a chunk's decays come to, by row.
-struct Decays {
+struct __align__(16) Decays {
     float enter[kChunk];      // e^{G_i} times the outputs' scale
     float leave[kChunk];      // e^{G_last - G_j} times the scale of k v^T; 0 for rows that are not there
-    int whole[kChunk];        // floor of G in base 2
-    float part[kChunk];       // and the rest
-    float all;                // e^{G_last}
+    float query[kChunk], key[kChunk];      // e^{G_i - G_a}, e^{G_a - G_j} with a the first visit of the row's half of the chunk
+    float far[kChunk];        // the same about the last visit of the first half, for queries of the second and keys of the first
+    int whole[kChunk];        // G in base 2
+    float part[kChunk];
+    float all, rest;          // e^{G_last}: the fp32 value nearest to it, and what that leaves
+    int gentle;               // query and key are fit for use
 };
 
-// One warp: the decays of visits s0 .. s0 + 63, two for each lane; returns the chunk's sum in base 2.
-__device__ __forceinline__ double chunk_decays(Decays *d, const Problem &p, int64_t b, int64_t h, int64_t s0, int64_t len, int lane) {
-    constexpr double kLog2e = 1.4426950408889634, kEmpty = -1048576.0;
-    double g[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int64_t s = s0 + 2 * lane + i;
-        g[i] = s < len ? (double)p.log_decay(b, h, s, len) * kLog2e : 0.0;
-        if (g[i] < kEmpty) g[i] = kEmpty;      // (a NaN stays one)
-    }
-    double sum = g[0] + g[1];
+// A sum of log decays in base 2: a whole number and a rest of a half at most, which keeps its own 24 bits.
+struct Log { int whole; float part; };
+__device__ __forceinline__ Log tidy(int whole, float part) {
+    const float r = rintf(part);
+    return {whole + (int)r, part - r};
+}
+__device__ __forceinline__ Log operator+(Log a, Log b) { return tidy(a.whole + b.whole, a.part + b.part); }
+__device__ __forceinline__ Log operator-(Log a, Log b) { return {a.whole - b.whole, a.part - b.part}; }
+__device__ __forceinline__ Log in_base_2(float g) {
+    constexpr float kLog2e = 1.44269504f, kRest = 1.92596299e-8f;      // log2(e) = the two together
+    const float high = g * kLog2e;
+    if (high < -1048576.f) return {-1048576, 0.f};      // (a NaN stays one, in the rest)
+    return tidy(0, high) + Log{0, fmaf(g, kLog2e, -high) + g * kRest};
+}
+__device__ __forceinline__ float power_of_2(int n) { return __int_as_float((min(max(n, -127), 128) + 127) << 23); }      // 0 below the normal range
+__device__ __forceinline__ float factor(Log x) { return exp2f(x.part) * power_of_2(x.whole); }
+
+// One warp's share of a chunk's decays: of visits s0 .. s0 + 63, two for each lane, whose logarithms were fetched ahead.
+// Returns the chunk's sum.  Every warp that takes part makes the sums; `part` 0 .. 2 says which factors it makes of them.
+constexpr int kDecayWarps = 3, kFirstDecayWarp = 5;
+__device__ __forceinline__ Log chunk_decays(Decays *d, const Problem &p, int part, int64_t s0, int64_t len, const float (&logs)[2], int lane) {
+    const Log g0 = in_base_2(logs[0]), g1 = in_base_2(logs[1]);
+    Log sum = g0 + g1;
 #pragma unroll
     for (int w = 1; w < 32; w <<= 1) {
-        const double x = __shfl_up_sync(0xffffffffu, sum, w);
-        if (lane >= w) sum += x;
+        const Log x{__shfl_up_sync(0xffffffffu, sum.whole, w), __shfl_up_sync(0xffffffffu, sum.part, w)};
+        if (lane >= w) sum = sum + x;
     }
-    const double last = __shfl_sync(0xffffffffu, sum, 31);
-    const double G[2] = {sum - g[1], sum};
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int visit = 2 * lane + i, row = p.reverse ? kChunk - 1 - visit : visit;
-        const bool there = s0 + visit < len;
-        const double whole = floor(G[i]);
-        d->whole[row] = (int)whole;
-        d->part[row] = (float)(G[i] - whole);
-        d->enter[row] = exp2f((float)G[i]) * p.out_scale;
-        d->leave[row] = there ? exp2f((float)(last - G[i])) * p.in_scale : 0.f;
+    const auto of_lane = [&](Log x, int from) { return Log{__shfl_sync(0xffffffffu, x.whole, from), __shfl_sync(0xffffffffu, x.part, from)}; };
+    const Log last = of_lane(sum, 31), G0 = sum - g1, G1 = sum;
+    const int row0 = p.reverse ? kChunk - 1 - 2 * lane : 2 * lane, row1 = p.reverse ? row0 - 1 : row0 + 1;
+    if (part == 0) {
+        d->enter[row0] = factor(G0) * p.out_scale;
+        d->enter[row1] = factor(G1) * p.out_scale;
+        d->leave[row0] = s0 + 2 * lane < len ? factor(last - G0) * p.in_scale : 0.f;
+        d->leave[row1] = s0 + 2 * lane + 1 < len ? factor(last - G1) * p.in_scale : 0.f;
+        if (lane == 0) {
+            // 1 + (2^part - 1), so that nothing of the second is lost
+            const float less = expm1f(last.part * 0.693147181f), all = 1.f + less, scale = power_of_2(last.whole);
+            d->all = all * scale;
+            d->rest = (less - (all - 1.f)) * scale;
+        }
+    } else if (part == 1) {
+        const Log first = of_lane(G0, lane & 16), x0 = G0 - first, x1 = G1 - first;
+        const bool gentle = __all_sync(0xffffffffu, abs(x0.whole) < 120 && abs(x1.whole) < 120);
+        d->query[row0] = factor(x0);
+        d->query[row1] = factor(x1);
+        d->key[row0] = factor(first - G0);
+        d->key[row1] = factor(first - G1);
+        if (lane == 0) d->gentle = gentle;
+    } else {
+        const Log middle = of_lane(sum, 15);
+        d->far[row0] = factor(lane < 16 ? middle - G0 : G0 - middle);
+        d->far[row1] = factor(lane < 16 ? middle - G1 : G1 - middle);
+        d->whole[row0] = G0.whole;
+        d->part[row0] = G0.part;
+        d->whole[row1] = G1.whole;
+        d->part[row1] = G1.part;
     }
-    if (lane == 0) d->all = exp2f((float)last);
     return last;
 }
 
 // x as the sum of `n` bf16 values, pairs packed
-template <int n> __device__ __forceinline__ void pieces(float x, float y, uint32_t (&w)[n]) {
+template <int n> __device__ __forceinline__ void pieces(Two xy, uint32_t (&w)[n]) {
 #pragma unroll
     for (int i = 0; i < n; ++i) {
+        float x, y;
+        split(xy, x, y);
         w[i] = umma::pack(x, y);
-        if (i + 1 < n) {
-            x -= umma::low(w[i]);
-            y -= umma::high(w[i]);
-        }
+        if (i + 1 < n) xy = fma2(two(umma::low(w[i]), umma::high(w[i])), splat(-1.f), xy);
     }
 }
+template <int n> __device__ __forceinline__ void pieces(float x, float y, uint32_t (&w)[n]) { pieces<n>(two(x, y), w); }
 
 __device__ __forceinline__ uint32_t unit_address(uint32_t base, int row, int channel) {      // of 8 channels, in the swizzle
     return base + channel / 64 * kPanel + row * 128 + ((channel % 64 / 8) ^ (row & 7)) * 16;
@@ -157,11 +193,11 @@ template <typename T, int n> __device__ __forceinline__ void load_rows(uint32_t 
     }
 }
 
-template <typename T, typename TO, int KD, int kLoad, int kInput, int kState, bool kOut>
+template <typename T, typename TO, int KD, int kLoad, int kInput, int kState, int kKeys, bool kOut>
 __global__ void __launch_bounds__(kThreads, kOut && kState > 1 ? 1 : kInput > 1 ? 1 : 2)
     chunked(Problem p, const __grid_constant__ Maps maps, Heads<const T> q, Heads<const T> k, Heads<const T> v, Heads<TO> o, int v_tiles, int flags,
             int32_t *status) {
-    using L = Plan<KD, kInput, kState, kOut>;
+    using L = Plan<KD, kInput, kState, kKeys, kOut>;
     extern __shared__ char raw[];
     __shared__ Decays decays[2];
     __shared__ __align__(8) uint64_t barriers[3];
@@ -176,7 +212,7 @@ __global__ void __launch_bounds__(kThreads, kOut && kState > 1 ? 1 : kInput > 1 
     id /= p.nseg;
     const int64_t h = id % p.H, b = id / p.H, len = p.length(b);
     const int Dv = min(p.Dv - vt * kValues, kValues);      // of this CTA
-    const bool vec = flags & 1, packed = sizeof(TO) == 2 && (flags & 2);
+    const bool vec = flags & 1, packed = sizeof(TO) == 2 && (flags & 2), boxed = kOut && kState == 1 && sizeof(TO) == 2 && (flags & 4);
     const int64_t begin = seg * p.seg_len, end = min((int64_t)p.T, begin + p.seg_len), stop = min(end, len);
     const int v_panels = Dv > 64 ? 2 : 1;
     const T *k_rows = k.row(b, 0, h), *q_rows = kOut ? q.row(b, 0, h) : nullptr, *v_rows = v.row(b, 0, h) + vt * kValues;
@@ -186,7 +222,9 @@ __global__ void __launch_bounds__(kThreads, kOut && kState > 1 ? 1 : kInput > 1 
 
     if (warp == 0) umma::tmem_alloc<L::kColumns>(umma::shared_address(&tmem_slot));
     if (threadIdx.x == 32) {
-        for (int i = 0; i < 3; ++i) umma::barrier_init(umma::shared_address(&barriers[i]), 1);
+        umma::barrier_init(loaded, kOut ? 3 : 2);
+        umma::barrier_init(scored, 1);
+        umma::barrier_init(added, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     // channels that no load writes
@@ -194,6 +232,13 @@ __global__ void __launch_bounds__(kThreads, kOut && kState > 1 ? 1 : kInput > 1 
         for (int i = threadIdx.x; i < kPanel / 16; i += kThreads) {
             const uint32_t zero[4] = {0, 0, 0, 0};
             store_shared16(base + L::kV + kPanel + i * 16, zero);
+        }
+
+    // scores above the diagonal: the half of them that no thread makes
+    if (kOut)
+        for (int i = threadIdx.x; i < kState * kPanel / 16; i += kThreads) {
+            const uint32_t zero[4] = {0, 0, 0, 0};
+            store_shared16(base + L::kP + i * 16, zero);
         }
 
     // the state that enters: lane = value channel, this half's key channels
@@ -239,15 +284,14 @@ __global__ void __launch_bounds__(kThreads, kOut && kState > 1 ? 1 : kInput > 1 
     const auto load = [&](int64_t s0) {
         const int64_t t0 = first_token(s0);
         if (kLoad == kTma) {
-            if (threadIdx.x == 64) {
-                umma::barrier_expect(loaded, (uint32_t)(((kOut ? 2 : 1) * L::kPanels + v_panels) * kPanel));
-                for (int c = 0; c < L::kPanels; ++c) {
-                    umma::tma_load(base + L::kK + c * kPanel, &maps.k, c * 64, k_head, (int)t0, (int)b, loaded);
-                    if (kOut) umma::tma_load(base + L::kQ + c * kPanel, &maps.q, c * 64, q_head, (int)t0, (int)b, loaded);
-                }
-                for (int c = 0; c < v_panels; ++c)
-                    umma::tma_load(base + L::kV + c * kPanel, &maps.v, vt * kValues + c * 64, v_head, (int)t0, (int)b, loaded);
-            }
+            // (a warp for each tensor: issuing takes a thread some hundred cycles)
+            const auto fetch = [&](const CUtensorMap *map, int to, int panels, int x, int head) {
+                umma::barrier_expect(loaded, (uint32_t)(panels * kPanel));
+                for (int c = 0; c < panels; ++c) umma::tma_load(base + to + c * kPanel, map, x + c * 64, head, (int)t0, (int)b, loaded);
+            };
+            if (threadIdx.x == 64) fetch(&maps.k, L::kK, L::kPanels, 0, k_head);
+            if (kOut && threadIdx.x == 96) fetch(&maps.q, L::kQ, L::kPanels, 0, q_head);
+            if (threadIdx.x == 128) fetch(&maps.v, L::kV, v_panels, vt * kValues, v_head);
         } else {
             const int there = (int)min((int64_t)kChunk, stop - s0), first = p.reverse ? kChunk - there : 0, last = p.reverse ? kChunk : there;
             load_rows<T, kInput>(base + L::kK, L::kKeyPiece, k_rows + t0 * k.st, k.st, first, last, p.Dk, KD, vec);
@@ -256,10 +300,20 @@ __global__ void __launch_bounds__(kThreads, kOut && kState > 1 ? 1 : kInput > 1 
         }
     };
 
-    double total = 0.0;      // warp 3: the logarithm of the decay of all chunks
+    const bool decayer = warp >= kFirstDecayWarp && warp < kFirstDecayWarp + kDecayWarps;
+    double total = 0.0;      // of these warps: the logarithm of the decay of all chunks
+    float logs[2];           // of the next chunk's decays
+    const auto fetch_logs = [&](int64_t s0) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) logs[i] = s0 + 2 * lane + i < len ? p.log_decay(b, h, s0 + 2 * lane + i, len) : 0.f;
+    };
     if (begin < stop) {
         load(begin);
-        if (warp == 3) total += chunk_decays(&decays[0], p, b, h, begin, len, lane);
+        if (decayer) {
+            fetch_logs(begin);
+            const Log x = chunk_decays(&decays[0], p, warp - kFirstDecayWarp, begin, len, logs, lane);
+            total += (double)x.whole + x.part;
+        }
         if (kOut) write_state();
     }
     umma::fence_async_shared();
@@ -275,6 +329,8 @@ __global__ void __launch_bounds__(kThreads, kOut && kState > 1 ? 1 : kInput > 1 
         const Decays &d = decays[parity];
         const int there = (int)min((int64_t)kChunk, stop - s0);      // tokens of the chunk
         const int64_t t0 = first_token(s0);
+        const bool full = there == kChunk;
+        if (decayer && s0 + kChunk < stop) fetch_logs(s0 + kChunk);
         if (kLoad == kTma) {
             const bool before = gave_up;
             umma::barrier_wait(loaded, parity, gave_up);
@@ -312,48 +368,77 @@ __global__ void __launch_bounds__(kThreads, kOut && kState > 1 ? 1 : kInput > 1 
                                             queries + ((c * L::kKeyPiece + s / 4 * kPanel + s % 4 * 32) >> 4), what, more);
             umma::tell_when_done(scored);
         }
-        // decayed keys: a unit of 8 channels of a row at a time, over the keys themselves once the scores are made
+        // Decayed keys, a unit of 8 channels of a row at a time.  The smaller pieces have room of their own; the first lies over
+        // the keys themselves, once the scores are made
         constexpr int kUnits = kChunk * KD / 8 / kThreads;
-        uint32_t unit[kUnits][kInput][4];
+        uint32_t first_piece[kUnits][4];
 #pragma unroll
         for (int i = 0; i < kUnits; ++i) {
             const int at = threadIdx.x + i * kThreads, row = at / (KD / 8), c = at % (KD / 8) * 8;
+            uint32_t unit[kInput][4], w[kKeys][4];
 #pragma unroll
-            for (int m = 0; m < kInput; ++m) load_shared16(unit_address(base + L::kK + m * L::kKeyPiece, row, c), unit[i][m]);
-        }
-        if (kOut) umma::barrier_wait(scored, parity, gave_up);
-        umma::after_sync();
-#pragma unroll
-        for (int i = 0; i < kUnits; ++i) {
-            const int at = threadIdx.x + i * kThreads, row = at / (KD / 8), c = at % (KD / 8) * 8;
-            const float f = d.leave[row];
-            const bool here = (p.reverse ? kChunk - 1 - row : row) < there;
-            uint32_t w[3][4];
+            for (int m = 0; m < kInput; ++m) load_shared16(unit_address(base + L::kK + m * L::kKeyPiece, row, c), unit[m]);
+            const Two f = splat(d.leave[row]);
+            const bool here = full || (p.reverse ? kChunk - 1 - row : row) < there;
+            if (kInput > 1 && kOut && i == 0) umma::barrier_wait(scored, parity, gave_up);      // all pieces lie over the keys'
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                float x = umma::low(unit[i][0][j]), y = umma::high(unit[i][0][j]);
-                if (kInput == 3) {      // (exact: the pieces do not overlap)
-                    x = (umma::low(unit[i][kInput - 1][j]) + umma::low(unit[i][kInput / 2][j])) + x;
-                    y = (umma::high(unit[i][kInput - 1][j]) + umma::high(unit[i][kInput / 2][j])) + y;
-                }
-                uint32_t z[3];
-                pieces<3>(here ? x * f : 0.f, here ? y * f : 0.f, z);
+                Two x = two(umma::low(unit[0][j]), umma::high(unit[0][j]));
+                if (kInput == 3)      // (exact: the pieces do not overlap)
+                    x = add2(x, add2(two(umma::low(unit[kInput - 1][j]), umma::high(unit[kInput - 1][j])),
+                                     two(umma::low(unit[kInput / 2][j]), umma::high(unit[kInput / 2][j]))));
+                uint32_t z[kKeys];
+                pieces<kKeys>(here ? mul2(x, f) : splat(0.f), z);
 #pragma unroll
-                for (int m = 0; m < 3; ++m) w[m][j] = z[m];
+                for (int m = 0; m < kKeys; ++m) w[m][j] = z[m];
+                first_piece[i][j] = z[0];
             }
 #pragma unroll
-            for (int m = 0; m < 3; ++m) store_shared16(unit_address(base + L::kK + m * L::kKeyPiece, row, c), w[m]);
+            for (int m = kInput > 1 ? 0 : 1; m < kKeys; ++m) store_shared16(unit_address(base + L::kK + m * L::kKeyPiece, row, c), w[m]);
         }
-        if (kOut && warp % 4 < 2) {
-            // scores: this thread's query, half of the keys
-            const int i = warp % 4 * 32 + lane;
-            const int whole = d.whole[i], visit = p.reverse ? kChunk - 1 - i : i;
-            const float part = d.part[i], scale = p.in_scale * p.out_scale;
+        if (kInput == 1) {
+            if (kOut) umma::barrier_wait(scored, parity, gave_up);
+#pragma unroll
+            for (int i = 0; i < kUnits; ++i) {
+                const int at = threadIdx.x + i * kThreads, row = at / (KD / 8), c = at % (KD / 8) * 8;
+                store_shared16(unit_address(base + L::kK, row, c), first_piece[i]);
+            }
+        }
+        umma::after_sync();
+        if (kOut && warp % 4 < 2 && (p.reverse ? half >= warp % 4 : half <= warp % 4)) {
+            // scores: this thread's query, a half of the keys
+            const int i = warp % 4 * 32 + lane, visit = p.reverse ? kChunk - 1 - i : i;
+            const bool same = half == warp % 4;
+            // the keys that count, by bits: all of an earlier half, those up to the query's own visit of the same one
+            uint32_t counts = !same ? 0xffffffffu : p.reverse ? 0xffffffffu << lane : 0xffffffffu >> (31 - lane);
+            if (visit >= there) counts = 0;
+            const float scale = p.in_scale * p.out_scale, mine = (same ? d.query[i] : d.far[i]) * scale;
+            const uint32_t theirs = umma::shared_address(same ? d.key : d.far) + half * 128;
+            const bool gentle = !same || d.gentle;
+            uint32_t both[2][16];
+            umma::tmem_load16(tmem + lanes + L::kScores + half * 32, both[0]);
+            umma::tmem_load16(tmem + lanes + L::kScores + half * 32 + 16, both[1]);
+            umma::tmem_wait_loads();
 #pragma unroll
             for (int j0 = 0; j0 < 32; j0 += 16) {
-                uint32_t r[16];
-                umma::tmem_load16(tmem + lanes + L::kScores + half * 32 + j0, r);
-                umma::tmem_wait_loads();
+                const uint32_t (&r)[16] = both[j0 / 16];
+                float decay[16];
+                if (gentle) {
+#pragma unroll
+                    for (int e = 0; e < 16; e += 4) {
+                        uint32_t x[4];
+                        load_shared16(theirs + (j0 + e) * 4, x);
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) decay[e + u] = __uint_as_float(x[u]) * mine;
+                    }
+                } else {
+                    asm volatile("" ::: "memory");      // (a branch of its own: not to be computed on the side)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const int j = half * 32 + j0 + e;
+                        decay[e] = factor(Log{d.whole[i], d.part[i]} - Log{d.whole[j], d.part[j]}) * scale;
+                    }
+                }
 #pragma unroll
                 for (int e = 0; e < 16; e += 8) {
                     uint32_t w[kState][4];
@@ -362,10 +447,8 @@ __global__ void __launch_bounds__(kThreads, kOut && kState > 1 ? 1 : kInput > 1 
                         float x[2];
 #pragma unroll
                         for (int u = 0; u < 2; ++u) {
-                            const int j = half * 32 + j0 + e + f + u, other = p.reverse ? kChunk - 1 - j : j;
-                            const int power = min(max(whole - d.whole[j], -127), 128);
-                            const float decay = umma::exp2_fast(part - d.part[j]) * __int_as_float((power + 127) << 23);
-                            x[u] = other <= visit && visit < there ? __uint_as_float(r[e + f + u]) * (decay * scale) : 0.f;
+                            const float y = __uint_as_float(r[e + f + u]) * decay[e + f + u];
+                            x[u] = counts & (1u << (j0 + e + f + u)) ? y : 0.f;
                         }
                         uint32_t y[kState];
                         pieces<kState>(x[0], x[1], y);
@@ -377,7 +460,7 @@ __global__ void __launch_bounds__(kThreads, kOut && kState > 1 ? 1 : kInput > 1 
                 }
             }
         }
-        if (warp == 3 && s0 + kChunk < stop) total += chunk_decays(&decays[parity ^ 1], p, b, h, s0 + kChunk, len, lane);
+        if (boxed && threadIdx.x == 64) umma::tma_wait_read();      // the chunk before this one's outputs
         umma::fence_async_shared();
         umma::before_sync();
         __syncthreads();
@@ -400,28 +483,63 @@ __global__ void __launch_bounds__(kThreads, kOut && kState > 1 ? 1 : kInput > 1 
 #pragma unroll
             for (int a = kInput - 1; a >= 0; --a)
 #pragma unroll
-                for (int c = 2; c >= 0; --c)
+                for (int c = kKeys - 1; c >= 0; --c)
 #pragma unroll
                     for (int s = 0; s < (a + c < 3 ? kChunk / 16 : 0); ++s, more = true)
                         umma::multiply(tmem + L::kAdded, values + ((a * L::kValuePiece + s * 2048) >> 4),
                                        decayed + ((c * L::kKeyPiece + s * 2048) >> 4), what, more);
             umma::tell_when_done(added);
         }
+        if (decayer && s0 + kChunk < stop) {
+            const Log x = chunk_decays(&decays[parity ^ 1], p, warp - kFirstDecayWarp, s0 + kChunk, len, logs, lane);
+            if (!kOut) total += (double)x.whole + x.part;
+        }
         umma::barrier_wait(added, parity, gave_up);
         umma::after_sync();
         if (s0 + kChunk < stop && !(kLoad == kTma && gave_up)) load(s0 + kChunk);
-        const float all = d.all;
+        const bool idle = warp % 4 * 32 >= Dv;      // this warp's value channels are padding
+        const Two all = splat(d.all), rest = splat(d.rest);
+        if (!idle) {
 #pragma unroll
-        for (int i = 0; i < kMine; i += 16) {
-            uint32_t r[16];
-            umma::tmem_load16(tmem + lanes + L::kAdded + key0 + i, r);
-            umma::tmem_wait_loads();
+            for (int i = 0; i < kMine; i += 32) {
+                uint32_t r[32];
+                umma::tmem_load16(tmem + lanes + L::kAdded + key0 + i, r);
+                umma::tmem_load16(tmem + lanes + L::kAdded + key0 + i + 16, r + 16);
+                umma::tmem_wait_loads();
 #pragma unroll
-            for (int j = 0; j < 16; ++j) state[i + j] = fmaf(all, state[i + j], __uint_as_float(r[j]));
+                for (int j = 0; j < 32; j += 2) {
+                    const Two old = two(state[i + j], state[i + j + 1]);
+                    split(fma2(all, old, fma2(rest, old, two(__uint_as_float(r[j]), __uint_as_float(r[j + 1])))), state[i + j], state[i + j + 1]);
+                }
+            }
         }
         if (kOut) {
-            if (s0 + kChunk < stop) write_state();
-            // outputs: lane = value channel, this half's 32 tokens
+            if (s0 + kChunk < stop && !idle) write_state();
+        }
+        if (kOut && !idle && boxed && full) {
+            // this half's 32 tokens, 16 value channels at a time: through shared memory, turned to rows of channels
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                uint32_t r1[16], r2[16];
+                umma::tmem_load_pairs32(tmem + lanes + ((uint32_t)u << 20) + L::kO1 + half * 32, r1);
+                umma::tmem_load_pairs32(tmem + lanes + ((uint32_t)u << 20) + L::kScores + half * 32, r2);
+                umma::tmem_wait_loads();
+                uint32_t w[4][2];
+#pragma unroll
+                for (int n = 0; n < 4; ++n) {
+                    const float2 e = *reinterpret_cast<const float2 *>(&d.enter[half * 32 + 8 * n + 2 * (lane % 4)]);
+#pragma unroll
+                    for (int c = 0; c < 2; ++c)
+                        w[n][c] = umma::pack(fmaf(e.x, __uint_as_float(r1[4 * n + 2 * c]), __uint_as_float(r2[4 * n + 2 * c])),
+                                             fmaf(e.y, __uint_as_float(r1[4 * n + 2 * c + 1]), __uint_as_float(r2[4 * n + 2 * c + 1])));
+                }
+#pragma unroll
+                for (int n = 0; n < 4; n += 2)
+                    umma::store_transposed(unit_address(base + L::kY, half * 32 + 8 * (n + lane / 16) + lane % 8, warp % 4 * 32 + u * 16 + lane / 8 % 2 * 8), w[n][0],
+                                           w[n][1], w[n + 1][0], w[n + 1][1]);
+            }
+        } else if (kOut && !idle) {
+            // lane = value channel, this half's 32 tokens
             TO *to = out + (t0 + half * 32) * o.st + (packed ? dv & ~1 : dv);
 #pragma unroll
             for (int i0 = 0; i0 < 32; i0 += 16) {
@@ -452,7 +570,12 @@ __global__ void __launch_bounds__(kThreads, kOut && kState > 1 ? 1 : kInput > 1 
         umma::before_sync();
         __syncthreads();
         umma::after_sync();
+        if (boxed && full && threadIdx.x == 64) {
+            for (int c = 0; c < v_panels; ++c) umma::tma_store(&maps.o, base + L::kY + c * kPanel, vt * kValues + c * 64, (int)h, (int)t0, (int)b);
+            umma::tma_commit();
+        }
     }
+    if (boxed && threadIdx.x == 64) umma::tma_wait_all();
     if (gave_up) report_status(status, FSS_STATUS_TMA_TIMEOUT);
     if (lost < 2) {      // copies that are still on their way: another two seconds before the CTA leaves its shared memory
         bool again = false;
@@ -466,7 +589,7 @@ __global__ void __launch_bounds__(kThreads, kOut && kState > 1 ? 1 : kInput > 1 
         float *to = kOut ? p.state_out + (b * p.H + h) * (int64_t)p.Dk * p.Dv : p.seg_state + ((b * p.H + h) * p.nseg + seg) * (int64_t)p.Dk * p.Dv;
         const int64_t sk = kOut ? p.sk : p.Dv, sv = kOut ? p.sv : 1;
         const float last = kOut && p.reverse && len > 0 ? expf(p.g[b * p.gsb + h * p.gsh]) : 1.f;
-        if (!kOut && vt == 0 && threadIdx.x == 96) p.seg_decay[(b * p.H + h) * p.nseg + seg] = (float)exp2(total);
+        if (!kOut && vt == 0 && threadIdx.x == kFirstDecayWarp * 32) p.seg_decay[(b * p.H + h) * p.nseg + seg] = (float)exp2(total);
 #pragma unroll
         for (int i = 0; i < kMine; ++i)
             if (dv < Dv && key0 + i < p.Dk) to[(key0 + i) * sk + (vt * kValues + dv) * sv] = state[i] * last;

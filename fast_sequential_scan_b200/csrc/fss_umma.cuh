@@ -54,6 +54,16 @@ __device__ __forceinline__ void tma_load(uint32_t to, const CUtensorMap *map, in
         : "memory");
 }
 
+// A box of shared memory into a tensor (what lies outside the tensor is dropped); no negative coordinates.
+__device__ __forceinline__ void tma_store(const CUtensorMap *map, uint32_t from, int x, int head, int token, int sequence) {
+    asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(map), "r"(from), "r"(x), "r"(head), "r"(token),
+                 "r"(sequence)
+                 : "memory");
+}
+__device__ __forceinline__ void tma_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void tma_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }      // shared memory may be written again
+__device__ __forceinline__ void tma_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
 // ------------------------------------------------------------------ tensor memory
 template <int kColumns> __device__ __forceinline__ void tmem_alloc(uint32_t slot) {      // a whole warp
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "n"(kColumns) : "memory");
@@ -73,6 +83,18 @@ __device__ __forceinline__ void tmem_load16(uint32_t at, uint32_t *r) {
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
                    "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
                  : "r"(at));
+}
+// 32 columns of 16 lanes: register 4 n + 2 u + e is lane t/4 + 8 u, column 8 n + 2 (t%4) + e of the thread t of the warp
+__device__ __forceinline__ void tmem_load_pairs32(uint32_t at, uint32_t *r) {
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+                   "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(at));
+}
+// four 8 x 8 matrices of 16-bit values, transposed on the way: thread t holds row t/4, columns 2 (t%4) and the next of
+// each; column c of matrix m goes to the 16 bytes that lane 8 m + c names
+__device__ __forceinline__ void store_transposed(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 __device__ __forceinline__ void tmem_store8(uint32_t at, const uint32_t *r) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
