@@ -30,6 +30,8 @@ from torch.autograd import Function
 from torch.autograd.function import once_differentiable
 
 from . import _lib, workspace
+from .scan_cuda import _ordinary_call
+from .sequential_scan_cuda import _fss_torch
 
 _DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float32: _lib.DTYPE_F32}
 MAX_DIM = 256      # of keys and of values
@@ -173,6 +175,10 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
     """Outputs ``[batch, seq, heads, value_dim]`` of whole sequences; with ``return_final_state`` also the fp32 state
     behind the last token, ``[batch, heads, key_dim, value_dim]``, which continues the sequence as the next call's
     ``h0``.  ``scale``: ``key_dim ** -0.5`` unless given.  See the module's docstring for layouts, decays and lengths."""
+    if _ordinary_call(*[t for t in (q, k, v, log_decay, h0, lengths) if t is not None]):
+        out = _fss_torch.attention(q, k, v, log_decay, h0, lengths, scale, bool(return_final_state))
+        if out is not None:
+            return out
     heads, K, V = _check_heads(q, k, v, log_decay, True)
     B, T = q.shape[:2]
     if h0 is not None:
@@ -202,6 +208,10 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log
     ``state``: fp32 ``[pool, heads, key_dim, value_dim]`` with contiguous states; sequence ``b`` has the entry ``slots[b]``
     (int32, on the device), or ``b`` without ``slots``.  A slot outside the pool (-1, say) marks a row of padding: its
     output is zeros and no state is touched.  Two sequences of a call must not share a slot.  Not differentiable."""
+    if _ordinary_call(*[t for t in (q, k, v, log_decay, state, slots) if t is not None]):
+        o = _fss_torch.attention_step(q, k, v, log_decay, state, scale, slots)
+        if o is not None:
+            return o
     heads, K, V = _check_heads(q, k, v, log_decay, False)
     B = q.shape[0]
     _check("state", state, 4, q, torch.float32)

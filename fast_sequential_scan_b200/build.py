@@ -1,5 +1,5 @@
 """In-tree build of ``libfss_b200.so`` (the C-ABI CUDA library) with plain nvcc for sm_100a, and of
-``_fss_torch*.so`` (the autograd side of the entry points, ``csrc/fss_torch.cpp``) with g++ against torch.
+``_fss_torch*.so`` (the autograd side of the entry points, ``csrc/fss_torch*.cpp``) with g++ against torch.
 The latter carries the Python and the torch it was compiled for in its name: one for another torch is neither
 taken for up to date here nor loaded by the package.
 
@@ -20,7 +20,7 @@ PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 OBJECTS = PKG / "build"      # one object for each .cu, with the list of what it was made from
 LIB = PKG / "libfss_b200.so"
-TORCH_SOURCE = CSRC / "fss_torch.cpp"
+TORCH_SOURCES = [CSRC / "fss_torch.cpp", CSRC / "fss_torch_layers.cpp"]
 
 NVCC_FLAGS = [
     "-O3", "-std=c++17",
@@ -49,25 +49,26 @@ def is_stale() -> bool:
 
 
 def torch_lib() -> Path:
-    """Where ``fss_torch.cpp`` is built for the running Python and torch."""
+    """Where ``fss_torch*.cpp`` are built for the running Python and torch."""
     import torch
     return PKG / f"_fss_torch.{sys.implementation.cache_tag}.torch-{torch.__version__}.so"
 
 
 def build_torch(force: bool = False) -> Path:
     lib = torch_lib()
-    inputs = [TORCH_SOURCE, PKG.parent / "include" / "fss_b200.h", Path(__file__)]
+    inputs = [*TORCH_SOURCES, CSRC / "fss_torch.h", PKG.parent / "include" / "fss_b200.h", Path(__file__)]
     if not force and lib.is_file() and lib.stat().st_mtime >= max(p.stat().st_mtime for p in inputs):
         return lib
     import sysconfig
 
     import torch
     root = Path(torch.__file__).resolve().parent
-    includes = [root / "include", root / "include" / "torch" / "csrc" / "api" / "include", Path(sysconfig.get_paths()["include"])]
+    includes = [root / "include", root / "include" / "torch" / "csrc" / "api" / "include", Path(sysconfig.get_paths()["include"]),
+                Path(_nvcc()).resolve().parent.parent / "include"]
     cmd = [shutil.which("g++") or "c++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
            "-DTORCH_EXTENSION_NAME=_fss_torch", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
-           *[f"-I{p}" for p in includes], str(TORCH_SOURCE), "-o", str(lib), f"-L{root / 'lib'}",
-           f"-Wl,-rpath,{root / 'lib'}", "-ltorch", "-ltorch_cpu", "-lc10", "-ltorch_python"]
+           *[f"-I{p}" for p in includes], *map(str, TORCH_SOURCES), "-o", str(lib), f"-L{root / 'lib'}",
+           f"-Wl,-rpath,{root / 'lib'}", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-ltorch_python"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode:
         sys.stderr.write(res.stdout + res.stderr)

@@ -10,13 +10,14 @@
 // workspaces stay with workspace.py: one Python call per launch takes the device's lock and returns what
 // the context is made of.  The GIL is held for such calls only, not for allocations, copies and launches,
 // any of which may block (memory to reclaim, a full launch queue).
-#include <torch/extension.h>
-
-#include "../../include/fss_b200.h"
+#include "fss_torch.h"
 
 namespace {
 
 using at::Tensor;
+using fss_torch::rowwise;
+using fss_torch::view;
+using fss_torch::like;
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
@@ -77,19 +78,6 @@ struct Launch {
     }
 };
 
-// unit channel stride, rows and batches that do not overlap
-Tensor rowwise(const Tensor &t) {
-    if (t.is_contiguous()) return t;
-    const int64_t B = t.size(0), T = t.size(1), D = t.size(2);
-    const bool ok = (D == 1 || t.stride(2) == 1) && (T == 1 || t.stride(1) >= D) && (B == 1 || t.stride(0) >= (T - 1) * t.stride(1) + D);
-    return ok ? t : t.contiguous();
-}
-fss_view view(const Tensor &t) {
-    const int64_t B = t.size(0), T = t.size(1), D = t.size(2);
-    if (t.is_contiguous()) return {t.data_ptr(), std::max<int64_t>(T * D, 1), D};
-    const int64_t st = T > 1 ? t.stride(1) : D;
-    return {t.data_ptr(), B > 1 ? t.stride(0) : std::max<int64_t>(st * T, 1), st};
-}
 // what the single-pass kernels can address
 bool addressable(const Tensor &t) {
     const int64_t per16 = 16 / t.element_size();
@@ -100,7 +88,6 @@ Tensor placed(const Tensor &t) {      // a copy where only the placement, not th
     if (t.size(2) % (16 / t.element_size()) || addressable(t)) return t;
     return t.clone(at::MemoryFormat::Contiguous);
 }
-Tensor like(const Tensor &t) { return at::empty(t.sizes(), t.options().memory_format(at::MemoryFormat::Contiguous)); }
 
 bool ordinary(const Tensor &t, const Tensor &first, at::ScalarType dtype) {
     return t.defined() && t.is_cuda() && t.layout() == at::kStrided && t.scalar_type() == dtype && t.dim() == 3 &&
@@ -244,4 +231,5 @@ PYBIND11_MODULE(_fss_torch, m) {
     m.def("bind", &bind);
     m.def("scan", &scan);
     m.def("gated", &gated);
+    fss_torch::define_layers(m);
 }

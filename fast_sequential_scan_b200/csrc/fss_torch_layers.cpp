@@ -1,0 +1,412 @@
+// Linear attention, rotary positions and the norm in C++ for ordinary calls, like the scans in fss_torch.cpp: each entry
+// returns None for a call it does not take, and the Python functions then do it, or word its refusal.
+//
+// What bounds the small calls is host time: one decoding step of 16 sequences runs 3 (positions, norm) to 12 us (20 heads'
+// states) of kernels; through ctypes a call took 27 us.
+#include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+
+#include "fss_torch.h"
+
+namespace {
+
+using at::Tensor;
+using fss_torch::like;
+using fss_torch::rowwise;
+using fss_torch::view;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+using Maybe = std::optional<Tensor>;
+
+struct Library {
+    decltype(&fss_linear_attention_workspace_bytes) attention_bytes;
+    decltype(&fss_linear_attention_forward) attention_forward;
+    decltype(&fss_linear_attention_backward) attention_backward;
+    decltype(&fss_linear_attention_step) attention_step;
+    decltype(&fss_rms_norm_forward) norm_forward;
+    decltype(&fss_rms_norm_workspace_bytes) norm_bytes;
+    decltype(&fss_rms_norm_backward) norm_backward;
+    decltype(&fss_rotary_apply) rotary;
+} lib;
+// Python: status_word(device index) -> address of the current stream's status word, after a look at it; check(code, where).
+// Held for the process's life.
+PyObject *py_status, *py_check;
+
+void check(int rc, const char *where) {
+    if (rc == FSS_OK) return;
+    py::gil_scoped_acquire gil;
+    py::reinterpret_borrow<py::object>(py_check)(rc, where);      // raises
+}
+
+fss_scan_ctx context(const Tensor &t, const Tensor &scratch, bool waits) {
+    fss_scan_ctx ctx{};
+    ctx.struct_bytes = sizeof(ctx);
+    ctx.device = t.get_device();
+    ctx.stream = c10::cuda::getCurrentCUDAStream(t.get_device()).stream();
+    if (scratch.defined()) {
+        ctx.workspace = scratch.data_ptr();
+        ctx.workspace_bytes = scratch.numel();
+    }
+    if (waits) {
+        py::gil_scoped_acquire gil;
+        ctx.status = reinterpret_cast<int32_t *>(py::reinterpret_borrow<py::object>(py_status)((int)t.get_device()).cast<uintptr_t>());
+    }
+    return ctx;
+}
+Tensor scratch(const Tensor &t, size_t bytes) { return bytes ? at::empty({(int64_t)bytes}, t.options().dtype(at::kByte)) : Tensor(); }
+
+int type_id(const Tensor &t) { return t.scalar_type() == at::kBFloat16 ? FSS_DTYPE_BF16 : FSS_DTYPE_F32; }
+bool ordinary(const Tensor &t, const Tensor &first) { return t.defined() && t.is_cuda() && t.layout() == at::kStrided && t.device() == first.device(); }
+bool supported(const Tensor &t) { return t.defined() && (t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kFloat) && ordinary(t, t); }
+bool neighbouring(const Tensor &t) { return t.size(-1) == 1 || t.stride(-1) == 1; }
+bool float_vector(const Tensor &t, const Tensor &first) { return ordinary(t, first) && t.scalar_type() == at::kFloat; }
+Tensor channels(const Tensor &t) { return neighbouring(t) ? t : t.contiguous(); }
+bool wants_grad(std::initializer_list<const Tensor *> all) {
+    if (!at::GradMode::is_enabled()) return false;
+    for (const Tensor *t : all)
+        if (t && t->defined() && t->requires_grad()) return true;
+    return false;
+}
+const Tensor none;
+const Tensor &given(const Maybe &t) { return t ? *t : none; }
+void *pointer(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+// What a backward returns has no derivative of its own; one that is asked for raises, as in the Python classes.
+variable_list once(variable_list grads) {
+    if (!at::GradMode::is_enabled()) return grads;
+    for (Tensor &g : grads)
+        if (g.defined()) {
+            Tensor x = g.detach();
+            x.set_requires_grad(true);
+            g = torch::autograd::DelayedError("trying to differentiate twice a function that was marked with @once_differentiable", 1)({x})[0];
+        }
+    return grads;
+}
+
+// ------------------------------------------------------------------ linear attention
+fss_heads heads(const Tensor &t) {
+    if (t.dim() == 3) return {t.data_ptr(), t.stride(0), 0, t.stride(1), t.size(1), t.size(2)};
+    return {t.data_ptr(), t.stride(0), t.stride(1), t.stride(2), t.size(2), t.size(3)};
+}
+
+// q, k, v that go together, with their decays; `dim` 4 or 3.  Returns the number of states, 0 for a call that is not ordinary.
+int64_t states(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &g, int64_t dim) {
+    if (!supported(q) || q.dim() != dim || q.numel() == 0) return 0;
+    for (const Tensor *t : {&k, &v}) {
+        if (!ordinary(*t, q) || t->scalar_type() != q.scalar_type() || t->dim() != dim || t->numel() == 0) return 0;
+        for (int64_t i = 0; i < dim - 2; ++i)
+            if (t->size(i) != q.size(i)) return 0;
+    }
+    if (k.size(-1) != q.size(-1) || q.size(-1) > 256 || v.size(-1) > 256) return 0;
+    const int64_t H = std::max({q.size(-2), k.size(-2), v.size(-2)});
+    if (H % q.size(-2) || H % k.size(-2) || H % v.size(-2) || !float_vector(g, q)) return 0;
+    if (g.dim() == 1) return g.size(0) == H ? H : 0;
+    if (g.dim() != dim - 1 || g.size(-1) != H) return 0;
+    for (int64_t i = 0; i < dim - 2; ++i)
+        if (g.size(i) != q.size(i)) return 0;
+    return H;
+}
+
+fss_linear_attention problem(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &g, const Tensor &h0, const Tensor &lengths, double scale, int64_t H,
+                             int64_t T) {
+    fss_linear_attention p{};
+    p.struct_bytes = sizeof(p);
+    p.dtype = type_id(q);
+    p.B = q.size(0);
+    p.T = T;
+    p.H = H;
+    p.q = heads(q);
+    p.k = heads(k);
+    p.v = heads(v);
+    p.log_decay = g.data_ptr<float>();
+    p.decay_stride_h = g.stride(-1);
+    if (g.dim() > 1) p.decay_stride_b = g.stride(0);
+    if (g.dim() > 2) p.decay_stride_t = g.stride(1);
+    p.lengths = lengths.defined() ? lengths.data_ptr<int32_t>() : nullptr;
+    p.h0 = h0.defined() ? h0.data_ptr<float>() : nullptr;
+    p.scale = (float)scale;
+    return p;
+}
+
+variable_list attention_forward(const Tensor &q_, const Tensor &k_, const Tensor &v_, const Tensor &g, const Tensor &h0, const Tensor &lengths, double scale,
+                                bool want_final) {
+    const Tensor q = channels(q_), k = channels(k_), v = channels(v_);
+    const int64_t B = q.size(0), T = q.size(1), H = std::max({q.size(2), k.size(2), v.size(2)}), K = q.size(3), V = v.size(3);
+    const Tensor o = at::empty({B, T, H, V}, v.options());
+    Tensor last;
+    if (want_final) last = at::empty({B, H, K, V}, v.options().dtype(at::kFloat));
+    const fss_linear_attention p = problem(q, k, v, g, h0, lengths, scale, H, T);
+    const Tensor room = scratch(q, lib.attention_bytes(&p, 0));
+    const fss_scan_ctx ctx = context(q, room, true);
+    const fss_heads out = heads(o);
+    check(lib.attention_forward(&ctx, &p, &out, static_cast<float *>(pointer(last))), "fss_linear_attention_forward");
+    if (want_final) return {o, last};
+    return {o};
+}
+
+struct Attention : torch::autograd::Function<Attention> {
+    static variable_list forward(AutogradContext *ctx, const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &g, const Maybe &h0, const Maybe &lengths,
+                                 double scale, bool want_final) {
+        const variable_list out = attention_forward(q, k, v, g, given(h0), given(lengths), scale, want_final);
+        ctx->set_materialize_grads(false);
+        ctx->save_for_backward({q, k, v, g, given(h0), given(lengths), want_final && g.requires_grad() ? out[1] : Tensor()});
+        ctx->saved_data["scale"] = scale;
+        return out;
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads) {
+        const variable_list saved = ctx->get_saved_variables();
+        const Tensor &g = saved[3], &h0 = saved[4], &lengths = saved[5], &last = saved[6];
+        const int64_t H = states(saved[0], saved[1], saved[2], g, 4);
+        TORCH_CHECK(H > 0, "linear_attention: a saved tensor came back with another shape, type or device");
+        const Tensor q = channels(saved[0]), k = channels(saved[1]), v = channels(saved[2]);
+        const int64_t B = q.size(0), T = q.size(1), K = q.size(3), V = v.size(3);
+        const auto state = [&](const Tensor &t) { return !t.defined() || (float_vector(t, q) && t.is_contiguous() && t.sizes() == at::IntArrayRef({B, H, K, V})); };
+        TORCH_CHECK(state(h0) && state(last) && (!lengths.defined() || (ordinary(lengths, q) && lengths.scalar_type() == at::kInt && lengths.is_contiguous() &&
+                                                                        lengths.numel() == B)),
+                    "linear_attention: a saved tensor came back with another shape, type or device");
+        const Tensor up = grads[0].defined() ? channels(grads[0]) : at::zeros({B, T, H, V}, v.options());
+        TORCH_CHECK(ordinary(up, q) && up.scalar_type() == v.scalar_type() && up.sizes() == at::IntArrayRef({B, T, H, V}),
+                    "linear_attention: the gradient has another shape, type or device than the output");
+        Tensor up_last;
+        if (grads.size() > 1 && grads[1].defined()) up_last = grads[1].contiguous();
+        TORCH_CHECK(state(up_last), "linear_attention: the last state's gradient has another shape, type or device than the state");
+        // (inputs that are not there have no number)
+        const bool decays = ctx->needs_input_grad(3), first = h0.defined() && ctx->needs_input_grad(4);
+        Tensor dq, dk, dv, dg, dh0;
+        if (ctx->needs_input_grad(0) || decays) dq = like(q);
+        if (ctx->needs_input_grad(1) || decays) dk = like(k);
+        if (ctx->needs_input_grad(2) || first) dv = like(v);
+        if (decays) dg = like(g);
+        if (first) dh0 = like(h0);
+        const fss_linear_attention p = problem(q, k, v, g, h0, lengths, ctx->saved_data["scale"].toDouble(), H, T);
+        const Tensor room = scratch(q, lib.attention_bytes(&p, decays ? 2 : 1));
+        const fss_scan_ctx call = context(q, room, true);
+        const fss_heads vu = heads(up), vq = dq.defined() ? heads(dq) : fss_heads{}, vk = dk.defined() ? heads(dk) : fss_heads{},
+                        vv = dv.defined() ? heads(dv) : fss_heads{};
+        check(lib.attention_backward(&call, &p, &vu, static_cast<float *>(pointer(last)), static_cast<float *>(pointer(up_last)), dq.defined() ? &vq : nullptr,
+                                     dk.defined() ? &vk : nullptr, dv.defined() ? &vv : nullptr, static_cast<float *>(pointer(dg)), g.dim() == 3,
+                                     static_cast<float *>(pointer(dh0))),
+              "fss_linear_attention_backward");
+        const auto asked = [&](int i, const Tensor &t) { return ctx->needs_input_grad(i) ? t : Tensor(); };
+        return once({asked(0, dq), asked(1, dk), asked(2, dv), dg, dh0, Tensor(), Tensor(), Tensor()});
+    }
+};
+
+py::object attention(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &g, const Maybe &h0, const Maybe &lengths, std::optional<double> scale,
+                     bool want_final) {
+    const int64_t H = states(q, k, v, g, 4);
+    if (!H) return py::none();
+    const int64_t B = q.size(0), K = q.size(3), V = v.size(3);
+    if (h0 && !(float_vector(*h0, q) && h0->is_contiguous() && h0->sizes() == at::IntArrayRef({B, H, K, V}))) return py::none();
+    if (lengths && !(ordinary(*lengths, q) && lengths->scalar_type() == at::kInt && lengths->is_contiguous() && lengths->sizes() == at::IntArrayRef({B})))
+        return py::none();
+    const double by = scale ? *scale : 1.0 / std::sqrt((double)K);
+    const variable_list out = [&] {
+        py::gil_scoped_release no_gil;
+        if (wants_grad({&q, &k, &v, &g, &given(h0)})) return Attention::apply(q, k, v, g, h0, lengths, by, want_final);
+        return attention_forward(q, k, v, g, given(h0), given(lengths), by, want_final);
+    }();
+    if (want_final) return py::make_tuple(out[0], out[1]);
+    return py::cast(out[0]);
+}
+
+py::object attention_step(const Tensor &q_, const Tensor &k_, const Tensor &v_, const Tensor &g, const Tensor &state, std::optional<double> scale, const Maybe &slots) {
+    const int64_t H = states(q_, k_, v_, g, 3);
+    if (!H || wants_grad({&q_, &k_, &v_, &g, &state})) return py::none();
+    const int64_t B = q_.size(0), K = q_.size(2), V = v_.size(2), pool = state.dim() == 4 ? state.size(0) : 0;
+    if (!float_vector(state, q_) || state.dim() != 4 || pool < 1 || state.size(1) != H || state.size(2) != K || state.size(3) != V) return py::none();
+    // contiguous states, apart from one another
+    if (!state.is_contiguous() && !((V == 1 || state.stride(3) == 1) && (K == 1 || state.stride(2) == V) && (H == 1 || state.stride(1) == K * V) &&
+                                    (pool == 1 || state.stride(0) >= H * K * V)))
+        return py::none();
+    if (slots ? !(ordinary(*slots, q_) && slots->scalar_type() == at::kInt && slots->is_contiguous() && slots->sizes() == at::IntArrayRef({B})) : pool < B)
+        return py::none();
+    const Tensor o = [&] {
+        py::gil_scoped_release no_gil;
+        const Tensor q = channels(q_), k = channels(k_), v = channels(v_), o = at::empty({B, H, V}, v.options());
+        const fss_linear_attention p = problem(q, k, v, g, none, none, scale ? *scale : 1.0 / std::sqrt((double)K), H, 1);
+        const fss_scan_ctx ctx = context(q, none, false);
+        const fss_heads out = heads(o);
+        check(lib.attention_step(&ctx, &p, &out, state.data_ptr<float>(), state.stride(0), pool, slots ? slots->data_ptr<int32_t>() : nullptr),
+              "fss_linear_attention_step");
+        return o;
+    }();
+    return py::cast(o);
+}
+
+// ------------------------------------------------------------------ rotary positions
+variable_list turn(const Tensor &q_, const Tensor &k_, const Tensor &positions, const Tensor &turns, bool interleaved, double magnitude, bool inverse) {
+    const Tensor q = channels(q_), k = k_.defined() ? channels(k_) : k_;
+    variable_list out{like(q)};
+    if (k.defined()) out.push_back(like(k));
+    fss_rotary r{};
+    r.struct_bytes = sizeof(r);
+    r.interleaved = interleaved;
+    r.inverse = inverse;
+    r.magnitude = (float)magnitude;
+    r.rotary_dim = 2 * turns.numel();
+    r.positions = positions.data_ptr<int64_t>();
+    r.position_stride_t = positions.stride(-1);
+    if (positions.dim() > 1) r.position_stride_b = positions.stride(0);
+    r.turns = turns.data_ptr<int64_t>();
+    const fss_scan_ctx ctx = context(q, none, false);
+    const fss_heads vq = heads(q), vk = k.defined() ? heads(k) : fss_heads{};
+    check(lib.rotary(&ctx, type_id(q), q.size(0), q.size(1), &vq, k.defined() ? &vk : nullptr, out[0].data_ptr(), k.defined() ? out[1].data_ptr() : nullptr, &r),
+          "fss_rotary_apply");
+    return out;
+}
+bool rotary_inputs(const Tensor &q, const Tensor &k, const Tensor &positions, const Tensor &turns) {
+    if (!supported(q) || q.dim() != 4 || q.numel() == 0) return false;
+    if (k.defined() && !(ordinary(k, q) && k.scalar_type() == q.scalar_type() && k.dim() == 4 && k.numel() > 0 && k.size(0) == q.size(0) && k.size(1) == q.size(1) &&
+                         k.size(3) == q.size(3)))
+        return false;
+    if (!ordinary(turns, q) || turns.scalar_type() != at::kLong || turns.dim() != 1 || !turns.is_contiguous() || turns.numel() < 1 || turns.numel() > 512 ||
+        2 * turns.numel() > q.size(3))
+        return false;
+    if (!ordinary(positions, q) || positions.scalar_type() != at::kLong) return false;
+    return positions.dim() == 1 ? positions.size(0) == q.size(1) : positions.dim() == 2 && positions.size(0) == q.size(0) && positions.size(1) == q.size(1);
+}
+
+struct Rotary : torch::autograd::Function<Rotary> {
+    static variable_list forward(AutogradContext *ctx, const Tensor &q, const Maybe &k, const Tensor &positions, const Tensor &turns, bool interleaved, double magnitude) {
+        ctx->save_for_backward({positions, turns});
+        ctx->saved_data["interleaved"] = interleaved;
+        ctx->saved_data["magnitude"] = magnitude;
+        return turn(q, given(k), positions, turns, interleaved, magnitude, false);
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads) {
+        const variable_list saved = ctx->get_saved_variables();
+        const Tensor second = grads.size() > 1 ? grads[1] : Tensor();
+        TORCH_CHECK(rotary_inputs(grads[0], second, saved[0], saved[1]), "rotary: a saved tensor or gradient came back with another shape, type or device");
+        variable_list out = turn(grads[0], second, saved[0], saved[1], ctx->saved_data["interleaved"].toBool(), ctx->saved_data["magnitude"].toDouble(), true);
+        return once({out[0], out.size() > 1 ? out[1] : Tensor(), Tensor(), Tensor(), Tensor(), Tensor()});
+    }
+};
+
+py::object rotary(const Tensor &q, const Maybe &k, const Tensor &positions, const Tensor &turns, bool interleaved, double magnitude) {
+    if (!rotary_inputs(q, given(k), positions, turns)) return py::none();
+    const variable_list out = [&] {
+        py::gil_scoped_release no_gil;
+        if (wants_grad({&q, &given(k)})) return Rotary::apply(q, k, positions, turns, interleaved, magnitude);
+        return turn(q, given(k), positions, turns, interleaved, magnitude, false);
+    }();
+    if (k) return py::make_tuple(out[0], out[1]);
+    return py::cast(out[0]);
+}
+
+// ------------------------------------------------------------------ norm
+Tensor rows(const Tensor &t) { return rowwise(t.dim() == 3 ? t : t.reshape({1, -1, t.size(-1)})); }
+bool norm_inputs(const Tensor &x, const Tensor &w, const Tensor &residual) {
+    if (!supported(x) || x.dim() < 1 || x.numel() == 0) return false;
+    if (!ordinary(w, x) || w.dim() != 1 || w.size(0) != x.size(-1) || !w.is_contiguous() || (w.scalar_type() != x.scalar_type() && w.scalar_type() != at::kFloat))
+        return false;
+    return !residual.defined() || (ordinary(residual, x) && residual.scalar_type() == x.scalar_type() && residual.sizes() == x.sizes());
+}
+
+// y (or the 8-bit values), s or x itself, r, scales
+variable_list norm_forward(const Tensor &x, const Tensor &w, const Tensor &residual, double eps, bool want_r, bool quantized, int64_t group) {
+    const Tensor y = at::empty(x.sizes(), x.options().dtype(quantized ? at::kFloat8_e4m3fn : x.scalar_type()).memory_format(at::MemoryFormat::Contiguous));
+    Tensor s, r, scales;
+    if (residual.defined()) s = like(x);
+    if (want_r) r = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
+    if (quantized) {
+        std::vector<int64_t> of(x.sizes().begin(), x.sizes().end() - 1);
+        if (group) of.push_back(x.size(-1) / group);
+        scales = at::empty(of, x.options().dtype(at::kFloat));
+    }
+    const Tensor rx = rows(x), rr = residual.defined() ? rows(residual) : residual, rs = s.defined() ? rows(s) : s;
+    const fss_view vx = view(rx), vr = rr.defined() ? view(rr) : fss_view{}, vs = rs.defined() ? view(rs) : fss_view{};
+    const fss_norm_weight weight{w.data_ptr(), type_id(w)};
+    fss_norm_output out{};
+    if (quantized) {
+        out.held = y.data_ptr();
+        out.scales = scales.data_ptr<float>();
+        out.group = (int32_t)group;
+    } else {
+        out.y = view(rows(y));
+    }
+    out.rstd = static_cast<float *>(pointer(r));
+    const fss_scan_ctx ctx = context(x, none, false);
+    check(lib.norm_forward(&ctx, type_id(x), rx.size(0), rx.size(1), rx.size(2), &vx, rr.defined() ? &vr : nullptr, &weight, (float)eps, rs.defined() ? &vs : nullptr, &out),
+          "fss_rms_norm_forward");
+    return {y, s.defined() ? s : x, r, scales};
+}
+
+struct Norm : torch::autograd::Function<Norm> {
+    static variable_list forward(AutogradContext *ctx, const Tensor &x, const Tensor &w, const Maybe &residual, double eps) {
+        const variable_list out = norm_forward(x, w, given(residual), eps, true, false, 0);
+        ctx->set_materialize_grads(false);
+        ctx->save_for_backward({out[1], w, out[2]});
+        if (residual) return {out[0], out[1]};
+        return {out[0]};
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads) {
+        const variable_list saved = ctx->get_saved_variables();
+        const Tensor &s = saved[0], &w = saved[1], &r = saved[2];
+        const Tensor up = grads[0].defined() ? grads[0] : at::zeros_like(s), up_s = grads.size() > 1 ? grads[1] : Tensor();
+        TORCH_CHECK(norm_inputs(s, w, up) && norm_inputs(s, w, up_s) && float_vector(r, s) && r.is_contiguous() && r.numel() * s.size(-1) == s.numel(),
+                    "rms_norm: a saved tensor or gradient came back with another shape, type or device");
+        const Tensor dx = like(s);
+        Tensor dw, room;
+        if (ctx->needs_input_grad(1)) {
+            dw = like(w);
+            room = scratch(s, lib.norm_bytes(s.size(-1)));
+        }
+        const Tensor rs = rows(s), ru = rows(up), ra = up_s.defined() ? rows(up_s) : up_s, rd = rows(dx);
+        const fss_view vs = view(rs), vu = view(ru), va = ra.defined() ? view(ra) : fss_view{}, vd = view(rd);
+        const fss_norm_weight weight{w.data_ptr(), type_id(w)};
+        const fss_scan_ctx call = context(s, room, false);
+        check(lib.norm_backward(&call, type_id(s), rs.size(0), rs.size(1), rs.size(2), &vs, &weight, r.data_ptr<float>(), &vu, ra.defined() ? &va : nullptr, &vd,
+                                pointer(dw)),
+              "fss_rms_norm_backward");
+        // (grads has a second entry where there is a residual)
+        return once({ctx->needs_input_grad(0) ? dx : Tensor(), dw, grads.size() > 1 && ctx->needs_input_grad(2) ? dx : Tensor(), Tensor()});
+    }
+};
+
+py::object norm(const Tensor &x, const Tensor &w, const Maybe &residual, double eps) {
+    if (!norm_inputs(x, w, given(residual))) return py::none();
+    const variable_list out = [&] {
+        py::gil_scoped_release no_gil;
+        if (wants_grad({&x, &w, &given(residual)})) return Norm::apply(x, w, residual, eps);
+        return norm_forward(x, w, given(residual), eps, false, false, 0);
+    }();
+    if (residual) return py::make_tuple(out[0], out[1]);
+    return py::cast(out[0]);
+}
+
+py::object norm_quantized(const Tensor &x, const Tensor &w, const Maybe &residual, double eps, int64_t group) {
+    if (!norm_inputs(x, w, given(residual)) || wants_grad({&x, &w, &given(residual)})) return py::none();
+    if (group && ((group != 32 && group != 64 && group != 128) || x.size(-1) % group)) return py::none();
+    const variable_list out = [&] {
+        py::gil_scoped_release no_gil;
+        return norm_forward(x, w, given(residual), eps, false, true, group);
+    }();
+    if (residual) return py::make_tuple(out[0], out[3], out[1]);
+    return py::make_tuple(out[0], out[3]);
+}
+
+void bind_layers(const std::vector<uintptr_t> &at, py::object status, py::object check_code) {
+    TORCH_CHECK(at.size() == 8, "bind_layers: eight addresses");
+    lib = {reinterpret_cast<decltype(lib.attention_bytes)>(at[0]),    reinterpret_cast<decltype(lib.attention_forward)>(at[1]),
+           reinterpret_cast<decltype(lib.attention_backward)>(at[2]), reinterpret_cast<decltype(lib.attention_step)>(at[3]),
+           reinterpret_cast<decltype(lib.norm_forward)>(at[4]),       reinterpret_cast<decltype(lib.norm_bytes)>(at[5]),
+           reinterpret_cast<decltype(lib.norm_backward)>(at[6]),      reinterpret_cast<decltype(lib.rotary)>(at[7])};
+    py_status = status.release().ptr();
+    py_check = check_code.release().ptr();
+}
+
+}  // namespace
+
+namespace fss_torch {
+
+void define_layers(py::module_ &m) {
+    m.def("bind_layers", &bind_layers);
+    m.def("attention", &attention);
+    m.def("attention_step", &attention_step);
+    m.def("rotary", &rotary);
+    m.def("norm", &norm);
+    m.def("norm_quantized", &norm_quantized);
+}
+
+}  // namespace fss_torch

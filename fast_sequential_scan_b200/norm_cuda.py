@@ -21,7 +21,8 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib, workspace
 from .attention_cuda import _DTYPES, _check, _pointer
-from .sequential_scan_cuda import _rowwise, _view
+from .scan_cuda import _ordinary_call
+from .sequential_scan_cuda import _fss_torch, _rowwise, _view
 
 GROUPS = (32, 64, 128)
 
@@ -113,6 +114,10 @@ class RmsNorm(Function):
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, *, residual: Optional[torch.Tensor] = None, eps: float = 1e-6):
     """``y``, or ``(y, s)`` with a ``residual``; see the module's docstring.  Differentiable with respect to ``x``,
     ``weight`` and ``residual``."""
+    if _ordinary_call(x, weight) and (residual is None or _ordinary_call(residual)):
+        out = _fss_torch.norm(x, weight, residual, eps)
+        if out is not None:
+            return out
     _check_inputs(x, weight, residual)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad)):
         return RmsNorm.apply(x, weight, residual, float(eps))
@@ -126,6 +131,10 @@ def rms_norm_quantized(x: torch.Tensor, weight: torch.Tensor, *, residual: Optio
     ``scales``: fp32, one a row (``x.shape[:-1]``), or with ``group`` (32, 64 or 128, a divisor of the channels) one for
     each group of channels (``[..., channels // group]``).  A row or group whose largest value is below 1e-30 keeps its
     zeros and loses what is smaller.  Not differentiable."""
+    if group != 0 and _ordinary_call(x, weight) and (residual is None or _ordinary_call(residual)):
+        out = _fss_torch.norm_quantized(x, weight, residual, eps, group or 0)
+        if out is not None:
+            return out
     _check_inputs(x, weight, residual)
     if group is not None and (group not in GROUPS or x.shape[-1] % group):
         raise ValueError(f"group={group}: expected one of {GROUPS} that divides {x.shape[-1]} channels")

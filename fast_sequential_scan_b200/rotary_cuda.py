@@ -20,6 +20,8 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib, workspace
 from .attention_cuda import _DTYPES, _channels, _check, _heads
+from .scan_cuda import _ordinary_call
+from .sequential_scan_cuda import _fss_torch
 
 LAYOUTS = ("half", "interleaved")
 MAX_ROTARY_DIM = 1024
@@ -111,6 +113,10 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
     ``q``, ``k``: ``[batch, seq, heads, dim]``, bf16 or fp32, any strides with neighbouring channels.  ``positions``: integers
     ``[seq]`` or ``[batch, seq]``, any values.  ``turns``, ``magnitude``: from :func:`rotary_turns`; ``2 * turns.numel()``
     channels of each head are turned."""
+    if layout in LAYOUTS and _ordinary_call(q, positions, turns) and (k is None or _ordinary_call(k)):
+        out = _fss_torch.rotary(q, k, positions, turns, layout == "interleaved", magnitude)
+        if out is not None:
+            return out
     _check("q", q, 4, None)
     if q.dtype not in _DTYPES:
         raise RuntimeError(f"q: unsupported dtype {q.dtype} (bf16 or fp32)")

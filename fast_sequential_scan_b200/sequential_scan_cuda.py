@@ -413,6 +413,9 @@ def _load_fss_torch():
         return None
     module.bind(_address("fss_scan_forward_ex"), _address("fss_scan_backward_ex"), _address("fss_scan_forward_gated"),
                 _address("fss_scan_backward_gated"), _acquire, workspace.launched, _lib.check, scan_backward_gated)
+    module.bind_layers([_address(f"fss_{name}") for name in (
+        "linear_attention_workspace_bytes", "linear_attention_forward", "linear_attention_backward", "linear_attention_step", "rms_norm_forward",
+        "rms_norm_workspace_bytes", "rms_norm_backward", "rotary_apply")], workspace.status_word, _lib.check)
     return module
 
 

@@ -61,6 +61,7 @@ class Workspace:
         self.replaced = []       # smaller buffers of before: CUDA graphs that were captured with them still write there
         self.contexts = {}       # what the library is handed, per (algo, flags); never changed once made (by the caller)
         self.status = torch.zeros(1, dtype=torch.int32).pin_memory()
+        self.status_address = self.status.data_ptr()
         self._flag = self.status.numpy()      # same memory, read without going through torch
         self.order = _order(device)
         self._event = None
@@ -161,9 +162,8 @@ def get_locked(device: torch.device, nbytes: int) -> Workspace:
     return ws
 
 
-def call_context(device: torch.device, scratch=None) -> _lib.ScanCtx:
-    """What the library is handed for a launch that waits for no other CTA: the current stream, its status word and the
-    call's own scratch (a tensor, or None).  Such launches are not ordered against those of other streams."""
+def _of_stream(device: torch.device) -> Workspace:
+    """The current stream's workspace as the owner of its status word, which is read; its memory is left alone."""
     index = device.index if device.index is not None else torch.cuda.current_device()
     stream = current_stream_handle(device)
     ws = _cache.get((index, stream))
@@ -175,8 +175,26 @@ def call_context(device: torch.device, scratch=None) -> _lib.ScanCtx:
     if ws._flag[0]:
         with ws.order.lock:
             ws.raise_if_flagged()
-    return _lib.ScanCtx(ctypes.sizeof(_lib.ScanCtx), index, stream, scratch.data_ptr() if scratch is not None else None,
+    return ws
+
+
+def call_context(device: torch.device, scratch=None) -> _lib.ScanCtx:
+    """What the library is handed for a launch that waits for no other CTA: the current stream, its status word and the
+    call's own scratch (a tensor, or None).  Such launches are not ordered against those of other streams."""
+    ws = _of_stream(device)
+    return _lib.ScanCtx(ctypes.sizeof(_lib.ScanCtx), ws.device.index, ws.stream_handle, scratch.data_ptr() if scratch is not None else None,
                         scratch.numel() if scratch is not None else 0, ws.status.data_ptr(), _lib.ALGO_AUTO, 0)
+
+
+_status_devices: dict = {}
+
+
+def status_word(index: int) -> int:
+    """Address of the status word of the current stream of device ``index``, for the C++ functions."""
+    device = _status_devices.get(index)
+    if device is None:
+        device = _status_devices[index] = torch.device("cuda", index)
+    return _of_stream(device).status_address
 
 
 def launched(ws: Workspace) -> None:
