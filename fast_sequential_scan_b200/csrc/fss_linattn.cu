@@ -105,6 +105,7 @@ static Problem make_problem(const fss_linear_attention *p, const Pass &s, const 
     x.sk = s.transposed ? 1 : x.Dv;
     x.sv = s.transposed ? x.Dk : 1;
     x.nseg = w.nseg; x.seg_len = w.seg_len;
+    x.folded = w.nseg > kFoldInside;
     x.seg_state = static_cast<float *>(scratch);
     x.seg_decay = x.seg_state + x.B * x.H * w.nseg * (int64_t)x.Dk * x.Dv;
     return x;
@@ -124,8 +125,8 @@ template <typename T, typename TO, int L> static int run_recurrent(const Problem
         FSS_CUDA(cudaFuncSetAttribute(outputs, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), "shared memory of a recurrent pass");
     }
     if (w.nseg > 1) {
-        sums<<<(unsigned)blocks, w.warps * 32, smem, stream>>>(x, q, k, v, out, w.v_tiles, vec);
-        fold_segments<<<(unsigned)(x.B * x.H * ceil_div((int64_t)x.Dk * x.Dv, 256)), 256, 0, stream>>>(x);
+        sums<<<(unsigned)(blocks / w.nseg * (w.nseg - 1)), w.warps * 32, smem, stream>>>(x, q, k, v, out, w.v_tiles, vec);
+        if (x.folded) fold_segments<<<(unsigned)(x.B * x.H * ceil_div((int64_t)x.Dk * x.Dv, 256)), 256, 0, stream>>>(x);
     }
     outputs<<<(unsigned)blocks, w.warps * 32, smem, stream>>>(x, q, k, v, out, w.v_tiles, vec);
     return launch_check("linear attention launch");
@@ -163,10 +164,15 @@ static int run_chunked(const Problem &x, const Plan &w, const Pass &s, const fss
     FSS_CUDA(cudaFuncSetAttribute(outputs, cudaFuncAttributeMaxDynamicSharedMemorySize, all), "shared memory of a chunked pass");
     if (w.nseg > 1) {
         FSS_CUDA(cudaFuncSetAttribute(sums, cudaFuncAttributeMaxDynamicSharedMemorySize, few), "shared memory of a chunked pass");
-        sums<<<(unsigned)blocks, mma::kThreads, few, stream>>>(x, maps, q, k, v, out, w.v_tiles, flags, status);
-        fold_segments<<<(unsigned)(x.B * x.H * ceil_div((int64_t)x.Dk * x.Dv, 256)), 256, 0, stream>>>(x);
+        sums<<<(unsigned)(blocks / w.nseg * (w.nseg - 1)), mma::kThreads, few, stream>>>(x, maps, q, k, v, out, w.v_tiles, flags, status);
+        if (x.folded)
+            FSS_CUDA(launch_dependent(fold_segments, dim3((unsigned)(x.B * x.H * ceil_div((int64_t)x.Dk * x.Dv, 256))), dim3(256), 0, stream, x),
+                     "fold of the segments");
+        FSS_CUDA(launch_dependent(outputs, dim3((unsigned)blocks), dim3(mma::kThreads), all, stream, x, maps, q, k, v, out, w.v_tiles, flags, status),
+                 "linear attention launch");
+    } else {
+        outputs<<<(unsigned)blocks, mma::kThreads, all, stream>>>(x, maps, q, k, v, out, w.v_tiles, flags, status);
     }
-    outputs<<<(unsigned)blocks, mma::kThreads, all, stream>>>(x, maps, q, k, v, out, w.v_tiles, flags, status);
     return launch_check("linear attention launch");
 }
 
@@ -236,9 +242,13 @@ static int run_gradient(const fss_linear_attention *p, const Pass &s, const fss_
     const fss_heads o{each, p->T * p->H * D, p->H * D, D, p->H, D};
     const int rc = run_pass<T, float>(p, s, &o, dots != nullptr, scratch, status, stream);
     if (rc) return rc;
-    const int64_t blocks = ceil_div(p->B * p->T * x.heads, 8);
-    if (blocks > INT32_MAX) return FSS_E_SHAPE;
-    finish_gradient<T><<<(unsigned)blocks, 256, 0, stream>>>(p->B, p->T, p->H, x.heads, (int)D, each, make_heads<const T>(&x, p->H), make_heads<T>(dx, p->H), dots);
+    const int64_t rows = p->B * p->T * x.heads, blocks = ceil_div(rows, 8);
+    if (rows > INT32_MAX) return FSS_E_SHAPE;
+    if (blocks > 0) {
+        auto *finish = D % 4 == 0 ? finish_gradient<T, 4> : finish_gradient<T, 1>;
+        finish<<<(unsigned)blocks, 256, 0, stream>>>((unsigned)p->T, (unsigned)p->H, (unsigned)x.heads, (int)D, each, make_heads<const T>(&x, p->H),
+                                                     make_heads<T>(dx, p->H), dots, (unsigned)rows);
+    }
     return launch_check("linear attention gradient launch");
 }
 

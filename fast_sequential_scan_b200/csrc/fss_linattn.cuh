@@ -11,9 +11,10 @@
 // so that one operator serves the forward and its three gradients.  Rows from len to T are never read; their outputs
 // are zeros.
 //
-// A long sequence is cut into segments that run at the same time: a first launch takes every segment's own sum
-// (its state from an empty one) and decay, a second folds them in order into the state that enters each segment, a
-// third computes the outputs.  No CTA waits for another.
+// A long sequence is cut into segments that run at the same time: a first launch takes the own sum (the state from an empty
+// one) and decay of every segment but the last, and the launch that computes the outputs folds those before its own
+// segment, in order, into the state that enters it.  Of more than kFoldInside segments the fold is a launch of its own,
+// which leaves the entering states in place of the sums.  No CTA waits for another.
 //
 // This file: the definitions that all linear-attention kernels share, and the recurrent kernels, which take one token
 // after the other with the state in registers, in fp32 throughout: any head dimension up to 256, any strides, both
@@ -26,6 +27,7 @@ namespace fss {
 namespace linattn {
 
 constexpr int kMaxDim = 256;      // of keys and values
+constexpr int kFoldInside = 8;    // segments (a CTA of the outputs then reads up to seven states; the launch between costs 5 us and 12 bytes an element)
 constexpr int kShort = 16;        // tokens up to which the recurrent kernels take every call
 
 template <typename T> struct Heads {
@@ -37,6 +39,12 @@ template <typename T> struct Heads {
 
 template <typename T> inline Heads<T> make_heads(const fss_heads *x, int64_t H) {
     return Heads<T>{reinterpret_cast<T *>(x->ptr), x->stride_b, x->stride_t, x->stride_h, x->heads ? H / x->heads : 1};
+}
+
+__device__ __forceinline__ float load_fresh(const float *p) {
+    float x[1];
+    fss::load_fresh(p, x);
+    return x[0];
 }
 
 struct Problem {
@@ -52,8 +60,9 @@ struct Problem {
     int64_t sk, sv;
     int nseg;
     int64_t seg_len;         // tokens a segment
-    float *seg_state;        // [B, H, nseg] matrices [Dk, Dv]: a segment's own sum, later the state that enters it
+    float *seg_state;        // [B, H, nseg] matrices [Dk, Dv]: a segment's own sum, or, folded, the state that enters it
     float *seg_decay;        // [B, H, nseg]
+    bool folded;
 
     __device__ __forceinline__ int64_t length(int64_t b) const {
         if (!lengths) return T;
@@ -69,6 +78,36 @@ struct Problem {
         return g[b * gsb + t * gst + h * gsh];
     }
 };
+
+// ------------------------------------------------------------------ the state that enters a segment
+// N key channels from `key0` on of the value channel `value` of the state that enters segment `seg`, for the kernels that
+// compute outputs; zeros where there is no such channel.  What the launch before this one wrote is read past the L1.
+// Every load has an address that is there and no condition, so that sixteen of them travel together.
+template <int N> __device__ __forceinline__ void entering_state(const Problem &p, int64_t b, int64_t h, int seg, int key0, int value, float (&state)[N]) {
+    const int64_t bh = b * p.H + h, n = (int64_t)p.Dk * p.Dv;
+    const int count = value < p.Dv ? p.Dk - key0 : 0;      // channels that are there
+    const auto add = [&](const float *matrix, int64_t sk, int64_t sv, float decay) {
+        const float *from = matrix + (int64_t)min(value, p.Dv - 1) * sv;
+        constexpr int kBatch = N < 16 ? N : 16;
+#pragma unroll
+        for (int i0 = 0; i0 < N; i0 += kBatch) {
+            float x[kBatch];
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) x[i] = load_fresh(from + min(key0 + i0 + i, p.Dk - 1) * sk);
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) state[i0 + i] = i0 + i < count ? fmaf(decay, state[i0 + i], x[i]) : 0.f;
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < N; ++i) state[i] = 0.f;
+    const float *sums = p.seg_state + bh * p.nseg * n;
+    if (p.nseg > 1 && p.folded) {
+        add(sums + seg * n, p.Dv, 1, 0.f);
+        return;
+    }
+    if (p.state_in) add(p.state_in + bh * n, p.sk, p.sv, 0.f);
+    for (int j = 0; j < seg; ++j) add(sums + j * n, p.Dv, 1, load_fresh(p.seg_decay + bh * p.nseg + j));
+}
 
 // ------------------------------------------------------------------ recurrent kernels
 // One thread holds 32 x 4 elements of the state: 32 key channels of 4 value channels.  L lanes hold a value channel's
@@ -125,34 +164,23 @@ __global__ void __launch_bounds__(128) recurrent(Problem p, Heads<const T> q, He
     int64_t id = blockIdx.x;
     const int vt = id % v_tiles;
     id /= v_tiles;
-    const int seg = id % p.nseg;
-    id /= p.nseg;
+    const int segments = kOut ? p.nseg : p.nseg - 1;      // (nothing follows the last one's sum)
+    const int seg = id % segments;
+    id /= segments;
     const int64_t h = id % p.H, b = id / p.H, len = p.length(b);
     const int l = lane % L, group = lane / L;
     const int key0 = l * kLaneK, col0 = vt * tile + warp * S::kColumns + group * kLaneV;
 
     Two state[kLaneV][kLaneK / 2];
-    const float *from = nullptr;
-    int64_t sk = p.Dv, sv = 1;
-    if (p.nseg > 1) {
-        if (kOut) from = p.seg_state + ((b * p.H + h) * p.nseg + seg) * (int64_t)p.Dk * p.Dv;
-    } else if (p.state_in) {
-        from = p.state_in + (b * p.H + h) * (int64_t)p.Dk * p.Dv;
-        sk = p.sk;
-        sv = p.sv;
+#pragma unroll
+    for (int c = 0; c < kLaneV; ++c) {
+        float held[kLaneK];
+#pragma unroll
+        for (int i = 0; i < kLaneK; ++i) held[i] = 0.f;
+        if (kOut) entering_state(p, b, h, seg, key0, col0 + c, held);
+#pragma unroll
+        for (int i = 0; i < kLaneK / 2; ++i) state[c][i] = two(held[2 * i], held[2 * i + 1]);
     }
-#pragma unroll
-    for (int c = 0; c < kLaneV; ++c)
-#pragma unroll
-        for (int i = 0; i < kLaneK / 2; ++i) {
-            float e[2] = {0.f, 0.f};
-            if (from && col0 + c < p.Dv) {
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-                    if (key0 + 2 * i + j < p.Dk) e[j] = from[(key0 + 2 * i + j) * sk + (col0 + c) * sv];
-            }
-            state[c][i] = two(e[0], e[1]);
-        }
 
     const int64_t begin = seg * p.seg_len, end = min((int64_t)p.T, begin + p.seg_len);
     double total = 0.0;      // threads of the first warp: their share of the logarithm of the segment's decay
@@ -240,10 +268,11 @@ __global__ void __launch_bounds__(128) recurrent(Problem p, Heads<const T> q, He
     if (kOut) {
         const int64_t z0 = max(begin, len), columns = min(tile, p.Dv - vt * tile);
         for (int64_t i = threadIdx.x; i < (end - z0) * columns; i += blockDim.x) o.row(b, z0 + i / columns, h)[vt * tile + i % columns] = (TO)0.f;
-        if (p.nseg > 1 || !p.state_out) return;
+        if (seg != p.nseg - 1 || !p.state_out) return;
     }
     float *to;
     float last = 1.f;
+    int64_t sk, sv;
     if (kOut) {
         to = p.state_out + (b * p.H + h) * (int64_t)p.Dk * p.Dv;
         sk = p.sk;
@@ -270,32 +299,28 @@ __global__ void __launch_bounds__(128) recurrent(Problem p, Heads<const T> q, He
 
 // The segments' own sums, in order, into the states that enter them: in place, one thread for each state element.
 __global__ void __launch_bounds__(256) fold_segments(Problem p) {
-    const int64_t n = (int64_t)p.Dk * p.Dv, per = (n + blockDim.x - 1) / blockDim.x;
-    const int64_t bh = blockIdx.x / per, i = blockIdx.x % per * blockDim.x + threadIdx.x;
+    const unsigned n = (unsigned)(p.Dk * p.Dv), per = (n + blockDim.x - 1) / blockDim.x;
+    const unsigned bh = blockIdx.x / per, i = blockIdx.x % per * blockDim.x + threadIdx.x;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     if (i >= n) return;
-    const int64_t at = bh * n + i / p.Dv * p.sk + i % p.Dv * p.sv;
-    float *seg = p.seg_state + bh * p.nseg * n + i;
-    const float *decay = p.seg_decay + bh * p.nseg;
-    float s = p.state_in ? p.state_in[at] : 0.f;
+    float *seg = p.seg_state + (int64_t)bh * p.nseg * n + i;
+    const float *decay = p.seg_decay + (int64_t)bh * p.nseg;
+    float s = p.state_in ? p.state_in[(int64_t)bh * n + i / p.Dv * p.sk + i % p.Dv * p.sv] : 0.f;
     constexpr int kAhead = 8;      // in flight for each thread
     for (int j0 = 0; j0 < p.nseg; j0 += kAhead) {
         float own[kAhead], a[kAhead];
 #pragma unroll
         for (int j = 0; j < kAhead; ++j)
-            if (j0 + j < p.nseg) {
-                own[j] = seg[(j0 + j) * n];
-                a[j] = decay[j0 + j];
+            if (j0 + j < p.nseg - 1) {      // (the last segment has no sum)
+                own[j] = load_fresh(seg + (int64_t)(j0 + j) * n);
+                a[j] = load_fresh(decay + j0 + j);
             }
 #pragma unroll
         for (int j = 0; j < kAhead; ++j)
             if (j0 + j < p.nseg) {
-                seg[(j0 + j) * n] = s;
-                s = fmaf(a[j], s, own[j]);
+                seg[(int64_t)(j0 + j) * n] = s;
+                if (j0 + j < p.nseg - 1) s = fmaf(a[j], s, own[j]);
             }
-    }
-    if (p.state_out) {
-        const int64_t b = bh / p.H, h = bh % p.H;
-        p.state_out[at] = p.reverse && p.length(b) > 0 ? s * expf(p.g[b * p.gsb + h * p.gsh]) : s;
     }
 }
 
@@ -384,47 +409,64 @@ __global__ void __launch_bounds__(kStepThreads) step(int64_t B, int64_t H, int D
 // ------------------------------------------------------------------ gradients of shared heads, and of the decays
 // From the gradient of each state's own copy of a tensor, in fp32: the sum over the heads that share it, rounded once,
 // and the dot product of each copy with the tensor itself (what the decays' gradients are made of).  A warp for each
-// row of the tensor.
-template <typename T>
-__global__ void __launch_bounds__(256) finish_gradient(int64_t B, int64_t Tn, int64_t H, int64_t heads, int D, const float *each, Heads<const T> x, Heads<T> dx,
-                                                       float *dots) {
-    const int64_t row = (int64_t)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
+// row of the tensor, V neighbouring channels a lane; a row has at most two rounds of them.  Bound by memory.
+template <typename T, int V>
+__global__ void __launch_bounds__(256) finish_gradient(unsigned Tn, unsigned H, unsigned heads, int D, const float *each, Heads<const T> x, Heads<T> dx, float *dots,
+                                                       unsigned rows) {
+    const unsigned row = blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
     const int lane = threadIdx.x % 32;
-    if (row >= B * Tn * heads) return;
-    const int64_t hx = row % heads, bt = row / heads, b = bt / Tn, t = bt % Tn, group = H / heads;
-    const float *from = each + (bt * H + hx * group) * D;
-    const T *xr = x.row(b, t, hx * group);
-    T *out = dx.row(b, t, hx * group);
-    float total[kMaxDim / 32];
+    if (row >= rows) return;
+    const unsigned hx = row % heads, bt = row / heads, b = bt / Tn, t = bt % Tn, group = H / heads;
+    const float *from = each + ((int64_t)bt * H + hx * group) * D;
+    const T *xr = x.ptr + b * x.sb + t * x.st + hx * x.sh;
+    T *out = dx.ptr + b * dx.sb + t * dx.st + hx * dx.sh;
+    constexpr int kRounds = kMaxDim / (32 * V);
+    float total[kRounds][V], own[kRounds][V];
 #pragma unroll
-    for (int c = 0; c < kMaxDim / 32; ++c) total[c] = 0.f;
-    for (int64_t m = 0; m < group; ++m) {
+    for (int c = 0; c < kRounds; ++c)
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const int d = (c * 32 + lane) * V + i;
+            total[c][i] = 0.f;
+            own[c][i] = dots && d < D ? (float)xr[d] : 0.f;
+        }
+    for (unsigned m = 0; m < group; ++m) {
         float dot = 0.f;
 #pragma unroll
-        for (int c = 0; c < kMaxDim / 32; ++c) {
-            const int d = c * 32 + lane;
-            if (d < D) {
-                const float e = from[m * D + d];
-                total[c] += e;
+        for (int c = 0; c < kRounds; ++c) {
+            const int d = (c * 32 + lane) * V;
+            if (d >= D) continue;
+            float e[V];
+            if (V == 4) {
+                const float4 y = *reinterpret_cast<const float4 *>(from + (int64_t)m * D + d);
+                e[0] = y.x; e[1 % V] = y.y; e[2 % V] = y.z; e[3 % V] = y.w;
+            } else {
+                e[0] = from[(int64_t)m * D + d];
+            }
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                total[c][i] += e[i];
                 // (a row beyond the sequence's length has zeros for its gradient, and anything for itself)
-                if (dots && e != 0.f) dot = fmaf(e, (float)xr[d], dot);
+                if (e[i] != 0.f) dot = fmaf(e[i], own[c][i], dot);
             }
         }
         if (dots) {
             for (int w = 16; w; w >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, w);
-            if (lane == 0) dots[bt * H + hx * group + m] = dot;
+            if (lane == 0) dots[(int64_t)bt * H + hx * group + m] = dot;
         }
     }
 #pragma unroll
-    for (int c = 0; c < kMaxDim / 32; ++c)
-        if (c * 32 + lane < D) out[c * 32 + lane] = (T)total[c];
+    for (int c = 0; c < kRounds; ++c)
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if ((c * 32 + lane) * V + i < D) out[(c * 32 + lane) * V + i] = (T)total[c][i];
 }
 
 // dL/dg_t = F_t = F_{t+1} + q_t.dq_t - k_t.dk_t, from F = <last state, its gradient> behind the last token; 0 where the
-// decay is 0.  One CTA for each (sequence, head) walks the tokens from the last to the first, 256 at a time; sums in
-// fp64, because F is what large terms of both signs leave.
+// decay is 0.  One CTA for each (sequence, head) walks the tokens from the last to the first, kFlowThreads * kFlowTokens at
+// a time; sums in fp64, because F is what large terms of both signs leave.
 // per_token: writes F [B, T, H]; else the sums over the tokens, [B, H].
-constexpr int kFlowThreads = 256;
+constexpr int kFlowThreads = 256, kFlowTokens = 4;
 __global__ void __launch_bounds__(kFlowThreads) decay_gradient(Problem p, const float *q_dq, const float *k_dk, const float *last, const float *grad_last,
                                                                float *per_token, float *sums) {
     __shared__ double part[kFlowThreads / 32], value[kFlowThreads / 32];
@@ -443,35 +485,57 @@ __global__ void __launch_bounds__(kFlowThreads) decay_gradient(Problem p, const 
     double sum = 0.0;
     if (per_token)
         for (int64_t t = len + threadIdx.x; t < p.T; t += kFlowThreads) per_token[(b * p.T + t) * p.H + h] = 0.f;
-    for (int64_t s0 = 0; s0 < len; s0 += kFlowThreads) {
-        const int64_t s = s0 + threadIdx.x, t = len - 1 - s;
-        double x = 0.0;
-        bool zero = false;      // what came before this visit no longer counts behind it
-        if (s < len) {
-            const int64_t at = (b * p.T + t) * p.H + h;
-            x = (double)q_dq[at] - (double)k_dk[at];
-            if (expf(p.g[b * p.gsb + t * p.gst + h * p.gsh]) == 0.f) { x = 0.0; zero = true; }
+    for (int64_t s0 = 0; s0 < len; s0 += kFlowThreads * kFlowTokens) {
+        double x[kFlowTokens];
+        bool zero[kFlowTokens];      // what came before this visit no longer counts behind it
+#pragma unroll
+        for (int i = 0; i < kFlowTokens; ++i) {
+            const int64_t s = s0 + threadIdx.x * kFlowTokens + i, t = len - 1 - s;
+            x[i] = 0.0;
+            zero[i] = false;
+            if (s < len) {
+                const int64_t at = (b * p.T + t) * p.H + h;
+                x[i] = (double)q_dq[at] - (double)k_dk[at];
+                zero[i] = expf(p.g[b * p.gsb + t * p.gst + h * p.gsh]) == 0.f;
+            }
         }
+        // this thread's own tokens, then the threads' totals
+        double total = 0.0;
+        bool cuts = false;
+#pragma unroll
+        for (int i = 0; i < kFlowTokens; ++i) {
+            total = zero[i] ? 0.0 : total + x[i];
+            cuts |= zero[i];
+        }
+        double incl = total;
+        bool any = cuts;
         for (int w = 1; w < 32; w <<= 1) {
-            const double px = __shfl_up_sync(0xffffffffu, x, w);
-            const bool pz = __shfl_up_sync(0xffffffffu, (int)zero, w);
+            const double px = __shfl_up_sync(0xffffffffu, incl, w);
+            const bool pz = __shfl_up_sync(0xffffffffu, (int)any, w);
             if (lane >= w) {
-                if (!zero) x += px;
-                zero |= pz;
+                if (!any) incl += px;
+                any |= pz;
             }
         }
         __syncthreads();
-        if (lane == 31) { value[warp] = x; cut[warp] = zero; }
+        if (lane == 31) { value[warp] = incl; cut[warp] = any; }
+        const double before = __shfl_up_sync(0xffffffffu, incl, 1);
+        const bool before_any = __shfl_up_sync(0xffffffffu, (int)any, 1);
         __syncthreads();
         double enter = flow;
         for (int w = 0; w < kFlowThreads / 32; ++w) {
             if (w == warp) enter = flow;
             flow = cut[w] ? value[w] : flow + value[w];
         }
-        if (!zero) x += enter;
-        if (s < len) {
-            if (per_token) per_token[(b * p.T + t) * p.H + h] = (float)x;
-            sum += x;
+        if (lane > 0) enter = before_any ? before : enter + before;
+#pragma unroll
+        for (int i = 0; i < kFlowTokens; ++i) {
+            const int64_t s = s0 + threadIdx.x * kFlowTokens + i;
+            enter = zero[i] ? 0.0 : enter + x[i];
+            if (s < len) {
+                if (per_token) per_token[(b * p.T + len - 1 - s) * p.H + h] = (float)enter;
+                sum += enter;
+            }
         }
     }
     if (sums) {

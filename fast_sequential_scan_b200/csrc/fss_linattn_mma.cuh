@@ -91,7 +91,7 @@ __device__ __forceinline__ float factor(Log x) { return exp2f(x.part) * power_of
 // One warp's share of a chunk's decays: of visits s0 .. s0 + 63, two for each lane, whose logarithms were fetched ahead.
 // Returns the chunk's sum.  Every warp that takes part makes the sums; `part` 0 .. 2 says which factors it makes of them.
 constexpr int kDecayWarps = 3, kFirstDecayWarp = 5;
-__device__ __forceinline__ Log chunk_decays(Decays *d, const Problem &p, int part, int64_t s0, int64_t len, const float (&logs)[2], int lane) {
+__device__ __forceinline__ Log chunk_decays(Decays *d, const Problem &p, int part, int s0, int len, const float (&logs)[2], int lane) {
     const Log g0 = in_base_2(logs[0]), g1 = in_base_2(logs[1]);
     Log sum = g0 + g1;
 #pragma unroll
@@ -155,6 +155,13 @@ __device__ __forceinline__ void load_shared16(uint32_t at, uint32_t (&w)[4]) {
     asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
 }
 
+// A value that the compiler takes for a new one: what is derived from it is derived again in every chunk instead of being kept
+// in registers, which the state needs.
+__device__ __forceinline__ uint32_t fresh(uint32_t x) {
+    asm volatile("" : "+r"(x));
+    return x;
+}
+
 // The chunk's rows of one tensor by ordinary loads, in `n` pieces; zeros for channels and rows that are not there.
 template <typename T, int n> __device__ __forceinline__ void load_rows(uint32_t base, int piece, const T *x, int64_t stride, int first, int last, int D,
                                                                        int padded, bool vec) {
@@ -208,12 +215,14 @@ __global__ void __launch_bounds__(kThreads, kOut && kState > 1 ? 1 : kInput > 1 
     int64_t id = blockIdx.x;
     const int vt = id % v_tiles;
     id /= v_tiles;
-    const int seg = id % p.nseg;
-    id /= p.nseg;
-    const int64_t h = id % p.H, b = id / p.H, len = p.length(b);
+    const int segments = kOut ? p.nseg : p.nseg - 1;      // (nothing follows the last one's sum)
+    const int seg = id % segments;
+    id /= segments;
+    const int64_t h = id % p.H, b = id / p.H;
+    const int len = (int)p.length(b);      // (fewer than 2^31 tokens)
     const int Dv = min(p.Dv - vt * kValues, kValues);      // of this CTA
     const bool vec = flags & 1, packed = sizeof(TO) == 2 && (flags & 2), boxed = kOut && kState == 1 && sizeof(TO) == 2 && (flags & 4);
-    const int64_t begin = seg * p.seg_len, end = min((int64_t)p.T, begin + p.seg_len), stop = min(end, len);
+    const int begin = (int)(seg * p.seg_len), end = (int)min(p.T, begin + p.seg_len), stop = min(end, len);
     const int v_panels = Dv > 64 ? 2 : 1;
     const T *k_rows = k.row(b, 0, h), *q_rows = kOut ? q.row(b, 0, h) : nullptr, *v_rows = v.row(b, 0, h) + vt * kValues;
     const int k_head = (int)(h / k.group), q_head = kOut ? (int)(h / q.group) : 0, v_head = (int)(h / v.group);
@@ -245,18 +254,11 @@ __global__ void __launch_bounds__(kThreads, kOut && kState > 1 ? 1 : kInput > 1 
     constexpr int kMine = KD / 2;
     const int dv = (warp % 4) * 32 + lane, key0 = half * kMine;
     float state[kMine];
-    {
-        const float *from = nullptr;
-        int64_t sk = p.Dv, sv = 1;
-        if (p.nseg > 1) {
-            if (kOut) from = p.seg_state + ((b * p.H + h) * p.nseg + seg) * (int64_t)p.Dk * p.Dv;
-        } else if (p.state_in) {
-            from = p.state_in + (b * p.H + h) * (int64_t)p.Dk * p.Dv;
-            sk = p.sk;
-            sv = p.sv;
-        }
 #pragma unroll
-        for (int i = 0; i < kMine; ++i) state[i] = from && dv < Dv && key0 + i < p.Dk ? from[(key0 + i) * sk + (vt * kValues + dv) * sv] : 0.f;
+    for (int i = 0; i < kMine; ++i) state[i] = 0.f;
+    if (kOut) {
+        asm volatile("griddepcontrol.wait;" ::: "memory");      // the segments' sums are another launch's
+        entering_state(p, b, h, seg, key0, vt * kValues + dv, state);
     }
     umma::fence_async_shared();
     umma::before_sync();
@@ -280,9 +282,9 @@ __global__ void __launch_bounds__(kThreads, kOut && kState > 1 ? 1 : kInput > 1 
         }
         umma::tmem_wait_stores();
     };
-    const auto first_token = [&](int64_t s0) { return p.reverse ? len - s0 - kChunk : s0; };
-    const auto load = [&](int64_t s0) {
-        const int64_t t0 = first_token(s0);
+    const auto first_token = [&](int s0) { return p.reverse ? len - s0 - kChunk : s0; };
+    const auto load = [&](int s0) {
+        const int t0 = first_token(s0);
         if (kLoad == kTma) {
             // (a warp for each tensor: issuing takes a thread some hundred cycles)
             const auto fetch = [&](const CUtensorMap *map, int to, int panels, int x, int head) {
@@ -293,17 +295,17 @@ __global__ void __launch_bounds__(kThreads, kOut && kState > 1 ? 1 : kInput > 1 
             if (kOut && threadIdx.x == 96) fetch(&maps.q, L::kQ, L::kPanels, 0, q_head);
             if (threadIdx.x == 128) fetch(&maps.v, L::kV, v_panels, vt * kValues, v_head);
         } else {
-            const int there = (int)min((int64_t)kChunk, stop - s0), first = p.reverse ? kChunk - there : 0, last = p.reverse ? kChunk : there;
-            load_rows<T, kInput>(base + L::kK, L::kKeyPiece, k_rows + t0 * k.st, k.st, first, last, p.Dk, KD, vec);
-            if (kOut) load_rows<T, kInput>(base + L::kQ, L::kKeyPiece, q_rows + t0 * q.st, q.st, first, last, p.Dk, KD, vec);
-            load_rows<T, kInput>(base + L::kV, L::kValuePiece, v_rows + t0 * v.st, v.st, first, last, Dv, kValues, vec);
+            const int there = min(kChunk, stop - s0), first = p.reverse ? kChunk - there : 0, last = p.reverse ? kChunk : there;
+            load_rows<T, kInput>(base + L::kK, L::kKeyPiece, k_rows + (int64_t)t0 * k.st, k.st, first, last, p.Dk, KD, vec);
+            if (kOut) load_rows<T, kInput>(base + L::kQ, L::kKeyPiece, q_rows + (int64_t)t0 * q.st, q.st, first, last, p.Dk, KD, vec);
+            load_rows<T, kInput>(base + L::kV, L::kValuePiece, v_rows + (int64_t)t0 * v.st, v.st, first, last, Dv, kValues, vec);
         }
     };
 
     const bool decayer = warp >= kFirstDecayWarp && warp < kFirstDecayWarp + kDecayWarps;
     double total = 0.0;      // of these warps: the logarithm of the decay of all chunks
     float logs[2];           // of the next chunk's decays
-    const auto fetch_logs = [&](int64_t s0) {
+    const auto fetch_logs = [&](int s0) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) logs[i] = s0 + 2 * lane + i < len ? p.log_decay(b, h, s0 + 2 * lane + i, len) : 0.f;
     };
@@ -321,14 +323,11 @@ __global__ void __launch_bounds__(kThreads, kOut && kState > 1 ? 1 : kInput > 1 
     __syncthreads();
     umma::after_sync();
 
-    // operands (steps and pieces are added to the address field, in units of 16 bytes)
-    const uint64_t queries = umma::operand(base + L::kQ, 16), keys = umma::operand(base + L::kK, 16), values = umma::operand(base + L::kV, kPanel),
-                   scores = umma::operand(base + L::kP, 16), decayed = umma::operand(base + L::kK, kPanel);
     uint32_t parity = 0, lost = 2;      // lost: the phase whose copies did not come
-    for (int64_t s0 = begin; s0 < stop; s0 += kChunk, parity ^= 1) {
+    for (int s0 = begin; s0 < stop; s0 += kChunk, parity ^= 1) {
         const Decays &d = decays[parity];
-        const int there = (int)min((int64_t)kChunk, stop - s0);      // tokens of the chunk
-        const int64_t t0 = first_token(s0);
+        const int there = min(kChunk, stop - s0);      // tokens of the chunk
+        const int t0 = first_token(s0);
         const bool full = there == kChunk;
         if (decayer && s0 + kChunk < stop) fetch_logs(s0 + kChunk);
         if (kLoad == kTma) {
@@ -347,6 +346,9 @@ __global__ void __launch_bounds__(kThreads, kOut && kState > 1 ? 1 : kInput > 1 
         }
         if (kOut && threadIdx.x == 64) {
             constexpr uint32_t what = umma::product(128, kChunk, false, false);
+            // operands (steps and pieces are added to the address field, in units of 16 bytes)
+            const uint32_t from = fresh(base);
+            const uint64_t queries = umma::operand(from + L::kQ, 16), keys = umma::operand(from + L::kK, 16);
             bool more = false;
             // (small pieces first: what a sum in fp32 loses goes by its size)
 #pragma unroll
@@ -372,12 +374,13 @@ __global__ void __launch_bounds__(kThreads, kOut && kState > 1 ? 1 : kInput > 1 
         // the keys themselves, once the scores are made
         constexpr int kUnits = kChunk * KD / 8 / kThreads;
         uint32_t first_piece[kUnits][4];
+        const uint32_t k_base = fresh(base) + L::kK;
 #pragma unroll
         for (int i = 0; i < kUnits; ++i) {
             const int at = threadIdx.x + i * kThreads, row = at / (KD / 8), c = at % (KD / 8) * 8;
             uint32_t unit[kInput][4], w[kKeys][4];
 #pragma unroll
-            for (int m = 0; m < kInput; ++m) load_shared16(unit_address(base + L::kK + m * L::kKeyPiece, row, c), unit[m]);
+            for (int m = 0; m < kInput; ++m) load_shared16(unit_address(k_base + m * L::kKeyPiece, row, c), unit[m]);
             const Two f = splat(d.leave[row]);
             const bool here = full || (p.reverse ? kChunk - 1 - row : row) < there;
             if (kInput > 1 && kOut && i == 0) umma::barrier_wait(scored, parity, gave_up);      // all pieces lie over the keys'
@@ -394,14 +397,14 @@ __global__ void __launch_bounds__(kThreads, kOut && kState > 1 ? 1 : kInput > 1 
                 first_piece[i][j] = z[0];
             }
 #pragma unroll
-            for (int m = kInput > 1 ? 0 : 1; m < kKeys; ++m) store_shared16(unit_address(base + L::kK + m * L::kKeyPiece, row, c), w[m]);
+            for (int m = kInput > 1 ? 0 : 1; m < kKeys; ++m) store_shared16(unit_address(k_base + m * L::kKeyPiece, row, c), w[m]);
         }
         if (kInput == 1) {
             if (kOut) umma::barrier_wait(scored, parity, gave_up);
 #pragma unroll
             for (int i = 0; i < kUnits; ++i) {
                 const int at = threadIdx.x + i * kThreads, row = at / (KD / 8), c = at % (KD / 8) * 8;
-                store_shared16(unit_address(base + L::kK, row, c), first_piece[i]);
+                store_shared16(unit_address(k_base, row, c), first_piece[i]);
             }
         }
         umma::after_sync();
@@ -413,15 +416,13 @@ __global__ void __launch_bounds__(kThreads, kOut && kState > 1 ? 1 : kInput > 1 
             uint32_t counts = !same ? 0xffffffffu : p.reverse ? 0xffffffffu << lane : 0xffffffffu >> (31 - lane);
             if (visit >= there) counts = 0;
             const float scale = p.in_scale * p.out_scale, mine = (same ? d.query[i] : d.far[i]) * scale;
-            const uint32_t theirs = umma::shared_address(same ? d.key : d.far) + half * 128;
+            const uint32_t theirs = umma::shared_address(same ? d.key : d.far) + half * 128, p_base = fresh(base) + L::kP;
             const bool gentle = !same || d.gentle;
-            uint32_t both[2][16];
-            umma::tmem_load16(tmem + lanes + L::kScores + half * 32, both[0]);
-            umma::tmem_load16(tmem + lanes + L::kScores + half * 32 + 16, both[1]);
-            umma::tmem_wait_loads();
 #pragma unroll
             for (int j0 = 0; j0 < 32; j0 += 16) {
-                const uint32_t (&r)[16] = both[j0 / 16];
+                uint32_t r[16];
+                umma::tmem_load16(tmem + lanes + L::kScores + half * 32 + j0, r);
+                umma::tmem_wait_loads();
                 float decay[16];
                 if (gentle) {
 #pragma unroll
@@ -456,7 +457,7 @@ __global__ void __launch_bounds__(kThreads, kOut && kState > 1 ? 1 : kInput > 1 
                         for (int m = 0; m < kState; ++m) w[m][f / 2] = y[m];
                     }
 #pragma unroll
-                    for (int m = 0; m < kState; ++m) store_shared16(unit_address(base + L::kP + m * kPanel, i, half * 32 + j0 + e), w[m]);
+                    for (int m = 0; m < kState; ++m) store_shared16(unit_address(p_base + m * kPanel, i, half * 32 + j0 + e), w[m]);
                 }
             }
         }
@@ -466,6 +467,8 @@ __global__ void __launch_bounds__(kThreads, kOut && kState > 1 ? 1 : kInput > 1 
         __syncthreads();
         umma::after_sync();
         if (threadIdx.x == 64) {
+            const uint32_t from = fresh(base);
+            const uint64_t values = umma::operand(from + L::kV, kPanel), scores = umma::operand(from + L::kP, 16), decayed = umma::operand(from + L::kK, kPanel);
             bool more = false;
             if (kOut) {
                 constexpr uint32_t what = umma::product(kValues, kChunk, true, false);
@@ -518,29 +521,27 @@ __global__ void __launch_bounds__(kThreads, kOut && kState > 1 ? 1 : kInput > 1 
         }
         if (kOut && !idle && boxed && full) {
             // this half's 32 tokens, 16 value channels at a time: through shared memory, turned to rows of channels
+            const uint32_t y_base = fresh(base) + L::kY;
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                uint32_t r1[16], r2[16];
-                umma::tmem_load_pairs32(tmem + lanes + ((uint32_t)u << 20) + L::kO1 + half * 32, r1);
-                umma::tmem_load_pairs32(tmem + lanes + ((uint32_t)u << 20) + L::kScores + half * 32, r2);
+            for (int step = 0; step < 4; ++step) {
+                const int u = step / 2, i0 = half * 32 + step % 2 * 16;      // 16 channels x 16 tokens
+                uint32_t r1[8], r2[8], w[4];
+                umma::tmem_load_pairs16(tmem + lanes + ((uint32_t)u << 20) + L::kO1 + i0, r1);
+                umma::tmem_load_pairs16(tmem + lanes + ((uint32_t)u << 20) + L::kScores + i0, r2);
                 umma::tmem_wait_loads();
-                uint32_t w[4][2];
 #pragma unroll
-                for (int n = 0; n < 4; ++n) {
-                    const float2 e = *reinterpret_cast<const float2 *>(&d.enter[half * 32 + 8 * n + 2 * (lane % 4)]);
+                for (int n = 0; n < 2; ++n) {
+                    const float2 e = *reinterpret_cast<const float2 *>(&d.enter[i0 + 8 * n + 2 * (lane % 4)]);
 #pragma unroll
                     for (int c = 0; c < 2; ++c)
-                        w[n][c] = umma::pack(fmaf(e.x, __uint_as_float(r1[4 * n + 2 * c]), __uint_as_float(r2[4 * n + 2 * c])),
-                                             fmaf(e.y, __uint_as_float(r1[4 * n + 2 * c + 1]), __uint_as_float(r2[4 * n + 2 * c + 1])));
+                        w[2 * n + c] = umma::pack(fmaf(e.x, __uint_as_float(r1[4 * n + 2 * c]), __uint_as_float(r2[4 * n + 2 * c])),
+                                                  fmaf(e.y, __uint_as_float(r1[4 * n + 2 * c + 1]), __uint_as_float(r2[4 * n + 2 * c + 1])));
                 }
-#pragma unroll
-                for (int n = 0; n < 4; n += 2)
-                    umma::store_transposed(unit_address(base + L::kY, half * 32 + 8 * (n + lane / 16) + lane % 8, warp % 4 * 32 + u * 16 + lane / 8 % 2 * 8), w[n][0],
-                                           w[n][1], w[n + 1][0], w[n + 1][1]);
+                umma::store_transposed(unit_address(y_base, i0 + 8 * (lane / 16) + lane % 8, warp % 4 * 32 + u * 16 + lane / 8 % 2 * 8), w[0], w[1], w[2], w[3]);
             }
         } else if (kOut && !idle) {
             // lane = value channel, this half's 32 tokens
-            TO *to = out + (t0 + half * 32) * o.st + (packed ? dv & ~1 : dv);
+            TO *to = out + (int64_t)(t0 + half * 32) * o.st + (packed ? dv & ~1 : dv);
 #pragma unroll
             for (int i0 = 0; i0 < 32; i0 += 16) {
                 uint32_t r1[16], r2[16];
@@ -582,10 +583,10 @@ __global__ void __launch_bounds__(kThreads, kOut && kState > 1 ? 1 : kInput > 1 
         umma::barrier_wait(loaded, lost, again);
     }
     if (kOut) {
-        const int64_t z0 = max(begin, len);
-        for (int64_t i = threadIdx.x; i < (end - z0) * Dv; i += kThreads) out[(z0 + i / Dv) * o.st + i % Dv] = (TO)0.f;
+        const int z0 = max(begin, len);
+        for (int64_t i = threadIdx.x; i < (int64_t)(end - z0) * Dv; i += kThreads) out[(z0 + i / Dv) * o.st + i % Dv] = (TO)0.f;
     }
-    if (!kOut || (p.nseg == 1 && p.state_out)) {
+    if (!kOut || (seg == p.nseg - 1 && p.state_out)) {
         float *to = kOut ? p.state_out + (b * p.H + h) * (int64_t)p.Dk * p.Dv : p.seg_state + ((b * p.H + h) * p.nseg + seg) * (int64_t)p.Dk * p.Dv;
         const int64_t sk = kOut ? p.sk : p.Dv, sv = kOut ? p.sv : 1;
         const float last = kOut && p.reverse && len > 0 ? expf(p.g[b * p.gsb + h * p.gsh]) : 1.f;

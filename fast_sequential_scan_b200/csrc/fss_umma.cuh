@@ -84,11 +84,10 @@ __device__ __forceinline__ void tmem_load16(uint32_t at, uint32_t *r) {
                    "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
                  : "r"(at));
 }
-// 32 columns of 16 lanes: register 4 n + 2 u + e is lane t/4 + 8 u, column 8 n + 2 (t%4) + e of the thread t of the warp
-__device__ __forceinline__ void tmem_load_pairs32(uint32_t at, uint32_t *r) {
-    asm volatile("tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
-                   "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+// 16 columns of 16 lanes: register 4 n + 2 u + e is lane t/4 + 8 u, column 8 n + 2 (t%4) + e of the thread t of the warp
+__device__ __forceinline__ void tmem_load_pairs16(uint32_t at, uint32_t *r) {
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
                  : "r"(at));
 }
 // four 8 x 8 matrices of 16-bit values, transposed on the way: thread t holds row t/4, columns 2 (t%4) and the next of
