@@ -62,7 +62,7 @@ static Plan make_plan(int64_t B, int64_t T, int64_t H, int64_t Dk, int64_t Dv, b
         block = mma::kChunk;
         w.v_tiles = (int)ceil_div(Dv, mma::kValues);
         // one CTA a multiprocessor with three pieces of everything, else two
-        w.nseg = choose_segments(B * H * w.v_tiles, T, kPlannedSms * (fine ? 1 : 2), block, {0.5, 128.0, 256.0, 0.7});
+        w.nseg = choose_segments(B * H * w.v_tiles, T, kPlannedSms * (fine ? 1 : 2), block, {0.5, 128.0, 240.0, 100.0, 0.7});
     } else {
         block = kBlock;
         w.lanes = Dk <= 32 ? 1 : Dk <= 64 ? 2 : Dk <= 128 ? 4 : 8;
@@ -70,7 +70,7 @@ static Plan make_plan(int64_t B, int64_t T, int64_t H, int64_t Dk, int64_t Dv, b
         w.warps = (int)(ceil_div(Dv, columns) < 4 ? ceil_div(Dv, columns) : 4);
         w.v_tiles = (int)ceil_div(Dv, columns * w.warps);
         // two CTAs of four warps a multiprocessor (registers); a pass for the sums alone does two thirds of the work
-        w.nseg = choose_segments(B * H * w.v_tiles, T, kPlannedSms * (8 / w.warps), block, {0.67, 8.0, 16.0, 0.1});
+        w.nseg = choose_segments(B * H * w.v_tiles, T, kPlannedSms * (8 / w.warps), block, {0.67, 8.0, 16.0, 16.0, 0.1});
     }
     w.seg_len = ceil_div(ceil_div(T > 0 ? T : 1, block), w.nseg) * block;
     w.seg_bytes = w.nseg > 1 ? align_up((size_t)(B * H * w.nseg) * (size_t)(Dk * Dv + 1) * sizeof(float), 256) : 0;
@@ -152,15 +152,15 @@ static bool make_map(CUtensorMap *map, const fss_heads &x, int64_t B, int64_t T)
               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T, typename TO, int KD, int kLoad, int kInput, int kState, int kKeys>
+template <typename T, typename TO, int KD, int kLoad, int kInput, int kState, int kKeys, bool kBoxed>
 static int run_chunked(const Problem &x, const Plan &w, const Pass &s, const fss_heads *o, const mma::Maps &maps, int flags, int32_t *status, cudaStream_t stream) {
     const auto q = make_heads<const T>(&s.q, x.H), k = make_heads<const T>(&s.k, x.H), v = make_heads<const T>(&s.v, x.H);
     const auto out = make_heads<TO>(o, x.H);
     const int64_t blocks = x.B * x.H * w.nseg * w.v_tiles;
     if (blocks > INT32_MAX) return FSS_E_SHAPE;
-    constexpr int few = mma::Plan<KD, kInput, kState, kKeys, false>::kShared, all = mma::Plan<KD, kInput, kState, kKeys, true>::kShared;
-    auto *sums = mma::chunked<T, TO, KD, kLoad, kInput, kState, kKeys, false>;
-    auto *outputs = mma::chunked<T, TO, KD, kLoad, kInput, kState, kKeys, true>;
+    constexpr int few = mma::Plan<KD, kInput, kState, kKeys, false, false>::kShared, all = mma::Plan<KD, kInput, kState, kKeys, true, kBoxed>::kShared;
+    auto *sums = mma::chunked<T, TO, KD, kLoad, kInput, kState, kKeys, false, false>;
+    auto *outputs = mma::chunked<T, TO, KD, kLoad, kInput, kState, kKeys, true, kBoxed>;
     FSS_CUDA(cudaFuncSetAttribute(outputs, cudaFuncAttributeMaxDynamicSharedMemorySize, all), "shared memory of a chunked pass");
     if (w.nseg > 1) {
         FSS_CUDA(cudaFuncSetAttribute(sums, cudaFuncAttributeMaxDynamicSharedMemorySize, few), "shared memory of a chunked pass");
@@ -183,26 +183,26 @@ template <typename T, typename TO> static int run_pass(const fss_linear_attentio
     const Problem x = make_problem(p, s, w, scratch);
     if (w.matrix) {
         mma::Maps maps{};
-        const auto out = make_heads<TO>(o, x.H);
         const int vec = wide_rows(make_heads<const T>(&s.q, x.H), x.Dk) && wide_rows(make_heads<const T>(&s.k, x.H), x.Dk) &&
                         wide_rows(make_heads<const T>(&s.v, x.H), x.Dv);
-        const int packed = x.Dv % 2 == 0 && out.sb % 2 == 0 && out.st % 2 == 0 && out.sh % 2 == 0 && reinterpret_cast<uintptr_t>(out.ptr) % 4 == 0;
-        int flags = vec | packed << 1;
         const bool narrow = x.Dk <= 64;
-#define FSS_CHUNKED(LOAD, INPUT, STATE, KEYS)                                                                             \
-    (narrow ? run_chunked<T, TO, 64, LOAD, INPUT, STATE, KEYS>(x, w, s, o, maps, flags, status, stream)                   \
-            : run_chunked<T, TO, 128, LOAD, INPUT, STATE, KEYS>(x, w, s, o, maps, flags, status, stream))
+#define FSS_CHUNKED(...)                                                                                   \
+    (narrow ? run_chunked<T, TO, 64, __VA_ARGS__>(x, w, s, o, maps, vec, status, stream)                   \
+            : run_chunked<T, TO, 128, __VA_ARGS__>(x, w, s, o, maps, vec, status, stream))
         if constexpr (sizeof(T) == 4) {
-            return FSS_CHUNKED(mma::kPlain, 3, 3, 3);
+            return FSS_CHUNKED(mma::kPlain, 3, 3, 3, false);
         } else {
             const bool tma = make_map(&maps.q, s.q, x.B, x.T) && make_map(&maps.k, s.k, x.B, x.T) && make_map(&maps.v, s.v, x.B, x.T);
             if constexpr (sizeof(TO) == 4) {
-                if (fine) return tma ? FSS_CHUNKED(mma::kTma, 1, 3, 3) : FSS_CHUNKED(mma::kPlain, 1, 3, 3);
+                if (fine) return tma ? FSS_CHUNKED(mma::kTma, 1, 3, 3, false) : FSS_CHUNKED(mma::kPlain, 1, 3, 3, false);
+                if (s.exact_state || x.state_out) return tma ? FSS_CHUNKED(mma::kTma, 1, 1, 3, false) : FSS_CHUNKED(mma::kPlain, 1, 1, 3, false);
+                return tma ? FSS_CHUNKED(mma::kTma, 1, 1, 2, false) : FSS_CHUNKED(mma::kPlain, 1, 1, 2, false);
             } else {
-                if (make_map(&maps.o, *o, x.B, x.T)) flags |= 4;
+                // (where TMA cannot address one of the tensors, all go by ordinary accesses)
+                const bool boxed = tma && make_map(&maps.o, *o, x.B, x.T);
+                if (s.exact_state || x.state_out) return boxed ? FSS_CHUNKED(mma::kTma, 1, 1, 3, true) : FSS_CHUNKED(mma::kPlain, 1, 1, 3, false);
+                return boxed ? FSS_CHUNKED(mma::kTma, 1, 1, 2, true) : FSS_CHUNKED(mma::kPlain, 1, 1, 2, false);
             }
-            if (!s.exact_state && !x.state_out) return tma ? FSS_CHUNKED(mma::kTma, 1, 1, 2) : FSS_CHUNKED(mma::kPlain, 1, 1, 2);
-            return tma ? FSS_CHUNKED(mma::kTma, 1, 1, 3) : FSS_CHUNKED(mma::kPlain, 1, 1, 3);
         }
 #undef FSS_CHUNKED
     }

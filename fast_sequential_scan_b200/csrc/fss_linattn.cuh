@@ -27,7 +27,7 @@ namespace fss {
 namespace linattn {
 
 constexpr int kMaxDim = 256;      // of keys and values
-constexpr int kFoldInside = 8;    // segments (a CTA of the outputs then reads up to seven states; the launch between costs 5 us and 12 bytes an element)
+constexpr int kFoldInside = 4;    // segments (reading one more state takes a CTA of the outputs 4 us; the launch between takes 6 us and more)
 constexpr int kShort = 16;        // tokens up to which the recurrent kernels take every call
 
 template <typename T> struct Heads {
@@ -565,9 +565,9 @@ constexpr int kPlannedSms = 148;      // segment lengths are planned for this ma
 
 // How many segments a sequence is cut into: `units` CTAs take one segment each, `slots` of them run at a time.  Costs in
 // the time that a CTA takes for a token: the segments' own sums are `extra` of a pass; what a CTA does once (its
-// state, to begin with) is `once`; folding is `launch` and `fold` for each unit's segment.  The shortest total
-// wins.  A segment is a multiple of `block` tokens.
-struct SegmentCosts { double extra, once, launch, fold; };
+// state, to begin with) is `once`; the second launch is `launch`, and where folding takes a third, that is `third` and
+// `fold` for each unit's segment.  The shortest total wins.  A segment is a multiple of `block` tokens.
+struct SegmentCosts { double extra, once, launch, third, fold; };
 inline int choose_segments(int64_t units, int64_t T, int64_t slots, int64_t block, const SegmentCosts &c) {
     const int64_t blocks = T > 0 ? ceil_div(T, block) : 1;
     int best = 1;
@@ -576,7 +576,7 @@ inline int choose_segments(int64_t units, int64_t T, int64_t slots, int64_t bloc
         const int64_t per = ceil_div(blocks, n);
         if (n > 1 && ceil_div(blocks, per) != n) continue;      // (the same segments as a smaller n)
         const double pass = (double)ceil_div(units * n, slots) * ((double)(per * block) + c.once);
-        const double cost = n > 1 ? pass * (1.0 + c.extra) + c.launch + c.fold * (double)(units * n) : pass;
+        const double cost = n > 1 ? pass * (1.0 + c.extra) + c.launch + (n > kFoldInside ? c.third : 0.0) + c.fold * (double)(units * n) : pass;
         if (n == 1 || cost < least) { least = cost; best = n; }
     }
     return best;

@@ -38,13 +38,13 @@ constexpr int kValues = 128;                                           // value 
 // kLoad: how the tokens come into shared memory
 enum Load { kTma = 0, kPlain = 1 };
 
-template <int KD, int kInput, int kState, int kKeys, bool kOut> struct Plan {
+template <int KD, int kInput, int kState, int kKeys, bool kOut, bool kBoxed> struct Plan {
     static constexpr int kPanels = KD / 64;
     static constexpr int kKeyPiece = kPanels * kPanel, kValuePiece = 2 * kPanel;
     // Q first: its product reads 128 rows, of which the upper half lies behind its panels
     static constexpr int kQ = 0, kK = kQ + (kOut ? kInput * kKeyPiece : 0), kV = kK + (kKeys > kInput ? kKeys : kInput) * kKeyPiece, kP = kV + kInput * kValuePiece;
     static constexpr int kY = kP + (kOut ? kState * kPanel : 0);      // outputs on their way, one piece of bf16
-    static constexpr int kEnd = kY + (kOut && kState == 1 ? kValuePiece : 0);
+    static constexpr int kEnd = kY + (kBoxed ? kValuePiece : 0);
     static constexpr int kShared = kEnd + 1024;      // (the base is moved up to a multiple of 1,024)
     // tensor memory
     static constexpr int kO1 = 0, kScores = 64, kAdded = kOut ? 128 : 0;
@@ -162,49 +162,62 @@ __device__ __forceinline__ uint32_t fresh(uint32_t x) {
     return x;
 }
 
-// The chunk's rows of one tensor by ordinary loads, in `n` pieces; zeros for channels and rows that are not there.
-template <typename T, int n> __device__ __forceinline__ void load_rows(uint32_t base, int piece, const T *x, int64_t stride, int first, int last, int D,
-                                                                       int padded, bool vec) {
-    for (int i = threadIdx.x; i < kChunk * padded / 8; i += kThreads) {
-        const int row = i / (padded / 8), c = i % (padded / 8) * 8;
-        float f[8];
+// The chunk's rows of one tensor by ordinary loads, `padded` channels of them, in two steps so that all of a thread's loads
+// travel together (and beside other work): fetch into registers, then put into shared memory in pieces.  Zeros for channels and
+// rows that are not there.
+template <typename T, int kPadded> struct Rows {
+    static constexpr int kUnits = kChunk * kPadded / 8 / kThreads, V = VecWidth<T>::value, kRaw = 8 / V;
+    typename Frag<T, V>::Raw raw[kUnits][kRaw];      // units of 8 channels
+
+    __device__ __forceinline__ void fetch(const T *x, int64_t stride, int first, int last, int D, bool vec) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = 0.f;
-        if (row >= first && row < last && c < D) {
-            const T *at = x + row * stride + c;
-            if (vec && c + 8 <= D) {
-                constexpr int V = VecWidth<T>::value;
+        for (int i = 0; i < kUnits; ++i) {
+            const int at = threadIdx.x + i * kThreads, row = at / (kPadded / 8), c = at % (kPadded / 8) * 8;
+            const bool here = row >= first && row < last;
 #pragma unroll
-                for (int j = 0; j < 8; j += V) {
-                    float y[V];
-                    Frag<T, V>::load(at + j, y);
+            for (int j = 0; j < kRaw; ++j) {
+                raw[i][j] = {};
+                if (vec) {      // (D is a multiple of V)
+                    if (here && c + j * V < D) raw[i][j] = Frag<T, V>::load_raw(x + row * stride + c + j * V);
+                } else {
+                    T e[V];
 #pragma unroll
-                    for (int e = 0; e < V; ++e) f[j + e] = y[e];
+                    for (int m = 0; m < V; ++m) e[m] = here && c + j * V + m < D ? x[row * stride + c + j * V + m] : T(0.f);
+                    memcpy(&raw[i][j], e, sizeof(e));
                 }
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (c + j < D) f[j] = (float)at[j];
             }
         }
-        uint32_t w[n][4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            uint32_t y[n];
-            pieces<n>(f[2 * j], f[2 * j + 1], y);
-#pragma unroll
-            for (int m = 0; m < n; ++m) w[m][j] = y[m];
-        }
-#pragma unroll
-        for (int m = 0; m < n; ++m) store_shared16(unit_address(base + m * piece, row, c), w[m]);
     }
-}
+    template <int n> __device__ __forceinline__ void put(uint32_t base, int piece) const {
+#pragma unroll
+        for (int i = 0; i < kUnits; ++i) {
+            const int at = threadIdx.x + i * kThreads, row = at / (kPadded / 8), c = at % (kPadded / 8) * 8;
+            uint32_t w[n][4];
+            if constexpr (sizeof(T) == 2) {
+                static_assert(n == 1, "one piece is all of a bf16 value");
+                memcpy(w[0], raw[i], 16);
+            } else {
+                float f[8];
+                memcpy(f, raw[i], 32);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    uint32_t y[n];
+                    pieces<n>(f[2 * j], f[2 * j + 1], y);
+#pragma unroll
+                    for (int m = 0; m < n; ++m) w[m][j] = y[m];
+                }
+            }
+#pragma unroll
+            for (int m = 0; m < n; ++m) store_shared16(unit_address(base + m * piece, row, c), w[m]);
+        }
+    }
+};
 
-template <typename T, typename TO, int KD, int kLoad, int kInput, int kState, int kKeys, bool kOut>
+template <typename T, typename TO, int KD, int kLoad, int kInput, int kState, int kKeys, bool kOut, bool kBoxed>
 __global__ void __launch_bounds__(kThreads, kOut && kState > 1 ? 1 : kInput > 1 ? 1 : 2)
     chunked(Problem p, const __grid_constant__ Maps maps, Heads<const T> q, Heads<const T> k, Heads<const T> v, Heads<TO> o, int v_tiles, int flags,
             int32_t *status) {
-    using L = Plan<KD, kInput, kState, kKeys, kOut>;
+    using L = Plan<KD, kInput, kState, kKeys, kOut, kBoxed>;
     extern __shared__ char raw[];
     __shared__ Decays decays[2];
     __shared__ __align__(8) uint64_t barriers[3];
@@ -221,7 +234,8 @@ __global__ void __launch_bounds__(kThreads, kOut && kState > 1 ? 1 : kInput > 1 
     const int64_t h = id % p.H, b = id / p.H;
     const int len = (int)p.length(b);      // (fewer than 2^31 tokens)
     const int Dv = min(p.Dv - vt * kValues, kValues);      // of this CTA
-    const bool vec = flags & 1, packed = sizeof(TO) == 2 && (flags & 2), boxed = kOut && kState == 1 && sizeof(TO) == 2 && (flags & 4);
+    const bool vec = flags & 1;
+    static_assert(!kBoxed || (kOut && kState == 1 && sizeof(TO) == 2), "only outputs of bf16 go through shared memory");
     const int begin = (int)(seg * p.seg_len), end = (int)min(p.T, begin + p.seg_len), stop = min(end, len);
     const int v_panels = Dv > 64 ? 2 : 1;
     const T *k_rows = k.row(b, 0, h), *q_rows = kOut ? q.row(b, 0, h) : nullptr, *v_rows = v.row(b, 0, h) + vt * kValues;
@@ -283,6 +297,23 @@ __global__ void __launch_bounds__(kThreads, kOut && kState > 1 ? 1 : kInput > 1 
         umma::tmem_wait_stores();
     };
     const auto first_token = [&](int s0) { return p.reverse ? len - s0 - kChunk : s0; };
+    // by ordinary loads, in steps
+    Rows<T, KD> keys, queries;
+    Rows<T, kValues> values;
+    const auto fetch_keys = [&](int s0) {
+        const int t0 = first_token(s0), there = min(kChunk, stop - s0), first = p.reverse ? kChunk - there : 0, last = p.reverse ? kChunk : there;
+        keys.fetch(k_rows + (int64_t)t0 * k.st, k.st, first, last, p.Dk, vec);
+        if (kOut) queries.fetch(q_rows + (int64_t)t0 * q.st, q.st, first, last, p.Dk, vec);
+    };
+    const auto fetch_values = [&](int s0) {
+        const int t0 = first_token(s0), there = min(kChunk, stop - s0), first = p.reverse ? kChunk - there : 0, last = p.reverse ? kChunk : there;
+        values.fetch(v_rows + (int64_t)t0 * v.st, v.st, first, last, Dv, vec);
+    };
+    const auto put_keys = [&] {
+        keys.template put<kInput>(base + L::kK, L::kKeyPiece);
+        if (kOut) queries.template put<kInput>(base + L::kQ, L::kKeyPiece);
+    };
+    const auto put_values = [&] { values.template put<kInput>(base + L::kV, L::kValuePiece); };
     const auto load = [&](int s0) {
         const int t0 = first_token(s0);
         if (kLoad == kTma) {
@@ -295,10 +326,10 @@ __global__ void __launch_bounds__(kThreads, kOut && kState > 1 ? 1 : kInput > 1 
             if (kOut && threadIdx.x == 96) fetch(&maps.q, L::kQ, L::kPanels, 0, q_head);
             if (threadIdx.x == 128) fetch(&maps.v, L::kV, v_panels, vt * kValues, v_head);
         } else {
-            const int there = min(kChunk, stop - s0), first = p.reverse ? kChunk - there : 0, last = p.reverse ? kChunk : there;
-            load_rows<T, kInput>(base + L::kK, L::kKeyPiece, k_rows + (int64_t)t0 * k.st, k.st, first, last, p.Dk, KD, vec);
-            if (kOut) load_rows<T, kInput>(base + L::kQ, L::kKeyPiece, q_rows + (int64_t)t0 * q.st, q.st, first, last, p.Dk, KD, vec);
-            load_rows<T, kInput>(base + L::kV, L::kValuePiece, v_rows + (int64_t)t0 * v.st, v.st, first, last, Dv, kValues, vec);
+            fetch_keys(s0);
+            put_keys();
+            fetch_values(s0);
+            put_values();
         }
     };
 
@@ -461,7 +492,7 @@ __global__ void __launch_bounds__(kThreads, kOut && kState > 1 ? 1 : kInput > 1 
                 }
             }
         }
-        if (boxed && threadIdx.x == 64) umma::tma_wait_read();      // the chunk before this one's outputs
+        if (kBoxed && threadIdx.x == 64) umma::tma_wait_read();      // the chunk before this one's outputs
         umma::fence_async_shared();
         umma::before_sync();
         __syncthreads();
@@ -497,9 +528,19 @@ __global__ void __launch_bounds__(kThreads, kOut && kState > 1 ? 1 : kInput > 1 
             const Log x = chunk_decays(&decays[parity ^ 1], p, warp - kFirstDecayWarp, s0 + kChunk, len, logs, lane);
             if (!kOut) total += (double)x.whole + x.part;
         }
+        // fp32 rows travel while the products are made and the state and the outputs are seen to: there are registers for them
+        // where a multiprocessor has one CTA
+        constexpr bool kEarly = kLoad == kPlain && kInput > 1;
+        const bool more_to_come = s0 + kChunk < stop;
+        if (kEarly && more_to_come) fetch_keys(s0 + kChunk);
         umma::barrier_wait(added, parity, gave_up);
         umma::after_sync();
-        if (s0 + kChunk < stop && !(kLoad == kTma && gave_up)) load(s0 + kChunk);
+        if (kEarly && more_to_come) {
+            put_keys();
+            fetch_values(s0 + kChunk);
+        } else if (more_to_come && !(kLoad == kTma && gave_up)) {
+            load(s0 + kChunk);
+        }
         const bool idle = warp % 4 * 32 >= Dv;      // this warp's value channels are padding
         const Two all = splat(d.all), rest = splat(d.rest);
         if (!idle) {
@@ -519,7 +560,7 @@ __global__ void __launch_bounds__(kThreads, kOut && kState > 1 ? 1 : kInput > 1 
         if (kOut) {
             if (s0 + kChunk < stop && !idle) write_state();
         }
-        if (kOut && !idle && boxed && full) {
+        if (kBoxed && !idle) {
             // this half's 32 tokens, 16 value channels at a time: through shared memory, turned to rows of channels
             const uint32_t y_base = fresh(base) + L::kY;
 #pragma unroll
@@ -539,44 +580,52 @@ __global__ void __launch_bounds__(kThreads, kOut && kState > 1 ? 1 : kInput > 1 
                 }
                 umma::store_transposed(unit_address(y_base, i0 + 8 * (lane / 16) + lane % 8, warp % 4 * 32 + u * 16 + lane / 8 % 2 * 8), w[0], w[1], w[2], w[3]);
             }
-        } else if (kOut && !idle) {
+        } else if (kOut && !kBoxed && !idle) {
             // lane = value channel, this half's 32 tokens
-            TO *to = out + (int64_t)(t0 + half * 32) * o.st + (packed ? dv & ~1 : dv);
+            TO *to = out + (int64_t)(t0 + half * 32) * o.st + dv;
+            // rows of this half that are there
+            const int from = p.reverse ? kChunk - there - half * 32 : 0, until = p.reverse ? 32 : there - half * 32;
 #pragma unroll
             for (int i0 = 0; i0 < 32; i0 += 16) {
                 uint32_t r1[16], r2[16];
                 umma::tmem_load16(tmem + lanes + L::kO1 + half * 32 + i0, r1);
                 umma::tmem_load16(tmem + lanes + L::kScores + half * 32 + i0, r2);
                 umma::tmem_wait_loads();
+                const float4 *enter = reinterpret_cast<const float4 *>(&d.enter[half * 32 + i0]);
 #pragma unroll
-                for (int e = 0; e < 16; e += 2) {
-                    const int row = half * 32 + i0 + e;
-                    float x = fmaf(d.enter[row], __uint_as_float(r1[e]), __uint_as_float(r2[e]));
-                    float y = fmaf(d.enter[row + 1], __uint_as_float(r1[e + 1]), __uint_as_float(r2[e + 1]));
-                    const auto here = [&](int r) { return (p.reverse ? kChunk - 1 - r : r) < there; };
-                    if (packed) {
-                        // neighbouring lanes swap a token each, and store two channels of one
-                        const float z = __shfl_xor_sync(0xffffffffu, lane % 2 ? x : y, 1);
-                        const uint32_t w = lane % 2 ? umma::pack(z, y) : umma::pack(x, z);
-                        const int mine = row + lane % 2;
-                        if (here(mine) && dv < Dv) *reinterpret_cast<uint32_t *>(to + (i0 + e + lane % 2) * o.st) = w;
-                    } else if (dv < Dv) {
-                        if (here(row)) to[(i0 + e) * o.st] = (TO)x;
-                        if (here(row + 1)) to[(i0 + e + 1) * o.st] = (TO)y;
-                    }
+                for (int e = 0; e < 16; e += 4) {
+                    const float4 f = enter[e / 4];
+                    const float x[4] = {fmaf(f.x, __uint_as_float(r1[e]), __uint_as_float(r2[e])), fmaf(f.y, __uint_as_float(r1[e + 1]), __uint_as_float(r2[e + 1])),
+                                        fmaf(f.z, __uint_as_float(r1[e + 2]), __uint_as_float(r2[e + 2])),
+                                        fmaf(f.w, __uint_as_float(r1[e + 3]), __uint_as_float(r2[e + 3]))};
+#pragma unroll
+                    for (int u = 0; u < 4; ++u, to += o.st)
+                        if (dv < Dv && (full || (i0 + e + u >= from && i0 + e + u < until))) *to = (TO)x[u];
                 }
             }
         }
+        if (kEarly && more_to_come) put_values();
         umma::fence_async_shared();
         umma::before_sync();
         __syncthreads();
         umma::after_sync();
-        if (boxed && full && threadIdx.x == 64) {
-            for (int c = 0; c < v_panels; ++c) umma::tma_store(&maps.o, base + L::kY + c * kPanel, vt * kValues + c * 64, (int)h, (int)t0, (int)b);
-            umma::tma_commit();
+        if (kBoxed && full) {
+            if (threadIdx.x == 64) {
+                for (int c = 0; c < v_panels; ++c) umma::tma_store(&maps.o, base + L::kY + c * kPanel, vt * kValues + c * 64, (int)h, t0, (int)b);
+                umma::tma_commit();
+            }
+        } else if (kBoxed) {
+            // the last chunk of a sequence: the rows that are there, 16 bytes at a time
+            const int first = p.reverse ? kChunk - there : 0, units = (Dv + 7) / 8;
+            for (int i = threadIdx.x; i < there * units; i += kThreads) {
+                const int row = first + i / units, c = i % units * 8;
+                uint32_t w[4];
+                load_shared16(unit_address(base + L::kY, row, c), w);
+                *reinterpret_cast<uint4 *>(out + (int64_t)(t0 + row) * o.st + c) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
         }
     }
-    if (boxed && threadIdx.x == 64) umma::tma_wait_all();
+    if (kBoxed && threadIdx.x == 64) umma::tma_wait_all();
     if (gave_up) report_status(status, FSS_STATUS_TMA_TIMEOUT);
     if (lost < 2) {      // copies that are still on their way: another two seconds before the CTA leaves its shared memory
         bool again = false;
