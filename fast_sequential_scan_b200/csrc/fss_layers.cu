@@ -11,6 +11,9 @@ template <typename T> bool wide_view(const fss_view *v, int64_t B, int64_t Tn) {
     return !v || !v->ptr || (aligned16(v->ptr) && (Tn <= 1 || v->stride_t % V == 0) && (B <= 1 || v->stride_b % V == 0));
 }
 
+// Whether the rows of a tensor lie evenly, from one sequence to the next.
+inline bool even(const fss_view *v, int64_t B, int64_t Tn) { return !v || !v->ptr || B <= 1 || v->stride_b == Tn * v->stride_t; }
+
 // How a row is laid over threads: fragments a thread and threads a row.  Up to 4 fragments for each lane of a warp, a
 // warp takes a row by itself; else a CTA does, with as few fragments a thread as it has threads for.
 struct Layout { int fragments, threads; bool block; };
@@ -60,6 +63,7 @@ int run_norm(const fss_scan_ctx *ctx, int64_t B, int64_t Tn, int64_t D, const fs
     p.weight = weight->ptr;
     p.eps = eps;
     p.group = out->group;
+    if (even(x, B, Tn) && even(residual, B, Tn) && even(residual ? sum : nullptr, B, Tn) && even(&out->y, B, Tn)) { p.B = 1; p.T_ = B * Tn; }
     const bool wide = weight->dtype == FSS_DTYPE_F32;
     const bool vec = D % VecWidth<T>::value == 0 && wide_view<T>(x, B, Tn) && wide_view<T>(residual, B, Tn) && wide_view<T>(residual ? sum : nullptr, B, Tn) &&
                      wide_view<T>(&out->y, B, Tn) && aligned16(weight->ptr) && aligned16(out->held);
@@ -84,6 +88,7 @@ int run_norm_backward(const fss_scan_ctx *ctx, int64_t B, int64_t Tn, int64_t D,
     p.rstd = rstd;
     p.weight = weight->ptr;
     p.parts = dweight ? static_cast<float *>(ctx->workspace) : nullptr;
+    if (even(s, B, Tn) && even(dy, B, Tn) && even(dsum, B, Tn) && even(dx, B, Tn)) { p.B = 1; p.T_ = B * Tn; }
     const bool wide = weight->dtype == FSS_DTYPE_F32;
     const bool vec = D % V == 0 && wide_view<T>(s, B, Tn) && wide_view<T>(dy, B, Tn) && wide_view<T>(dsum, B, Tn) && wide_view<T>(dx, B, Tn) && aligned16(weight->ptr);
     cudaStream_t stream = (cudaStream_t)ctx->stream;
@@ -96,7 +101,7 @@ int run_norm_backward(const fss_scan_ctx *ctx, int64_t B, int64_t Tn, int64_t D,
     } else {
         const int per = w.block ? 1 : w.threads / 32;
         int64_t blocks = ceil_div(rows, per);
-        const int64_t most = w.block ? 148 * (1024 / w.threads) : kNormWalkers / per;
+        const int64_t most = w.block ? 148 * (1024 / w.threads > 1 ? 1024 / w.threads : 1) : kNormWalkers / per;
         if (blocks > most) blocks = most;
         parts = blocks * per < rows ? blocks * per : rows;
 #define FSS_NORM(N, BLOCK) norm::backward<T, N, BLOCK><<<(unsigned)blocks, w.threads, 0, stream>>>(p, wide)
@@ -153,10 +158,11 @@ int run_rotary(const fss_scan_ctx *ctx, int64_t B, int64_t Tn, const fss_heads *
     p.psb = r->position_stride_b; p.pst = r->position_stride_t;
     p.turns = r->turns;
     p.magnitude = r->magnitude;
-    const int64_t rows = B * Tn, per_token = heads * (vec ? (r->interleaved ? p.D / V : (p.D - p.R / 2) / V) : p.D - p.R / 2);
-    // about 2,048 items a CTA, and no more than 4,096 sines; a few tokens are shared by several CTAs instead
-    int64_t tokens = 2048 / (per_token > 0 ? per_token : 1), most = 4096 / (p.R / 2);
+    const int64_t rows = B * Tn, per_head = vec ? (r->interleaved ? p.D / V : (p.D - p.R / 2) / V) : p.D - p.R / 2, per_token = heads * per_head;
+    // about 4,096 items a CTA, and no more than 4,096 sines and kMaxTokens tokens; a few tokens are shared by several CTAs instead
+    int64_t tokens = 4096 / per_token, most = 4096 / (p.R / 2);
     if (tokens > most) tokens = most;
+    if (tokens > rotary::kMaxTokens) tokens = rotary::kMaxTokens;
     if (tokens > rows / (4 * 148)) tokens = rows / (4 * 148);
     p.tokens = (int)(tokens < 1 ? 1 : tokens);
     const int64_t groups = ceil_div(rows, p.tokens);
@@ -171,7 +177,7 @@ int run_rotary(const fss_scan_ctx *ctx, int64_t B, int64_t Tn, const fss_heads *
         if (r->interleaved) kernel = r->inverse ? rotary::rotate<T, V, true, true> : rotary::rotate<T, V, true, false>;
         else kernel = r->inverse ? rotary::rotate<T, V, false, true> : rotary::rotate<T, V, false, false>;
     } else {
-        if (r->interleaved) kernel = r->inverse ? rotary::rotate_pairs<T, true> : rotary::rotate_pairs<T, false>;
+        if (r->interleaved) kernel = r->inverse ? rotary::rotate<T, 1, true, true> : rotary::rotate<T, 1, true, false>;
         else kernel = r->inverse ? rotary::rotate<T, 1, false, true> : rotary::rotate<T, 1, false, false>;
     }
     kernel<<<blocks, rotary::kThreads, smem, stream>>>(p);

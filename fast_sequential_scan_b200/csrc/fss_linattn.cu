@@ -62,7 +62,8 @@ static Plan make_plan(int64_t B, int64_t T, int64_t H, int64_t Dk, int64_t Dv, b
         block = mma::kChunk;
         w.v_tiles = (int)ceil_div(Dv, mma::kValues);
         // one CTA a multiprocessor with three pieces of everything, else two
-        w.nseg = choose_segments(B * H * w.v_tiles, T, kPlannedSms * (fine ? 1 : 2), block, {0.5, 128.0, 240.0, 100.0, 0.7});
+        w.nseg = choose_segments(B * H * w.v_tiles, T, kPlannedSms * (fine ? 1 : 2), block,
+                                 fine ? SegmentCosts{0.5, 64.0, 80.0, 40.0, 0.35} : SegmentCosts{0.5, 128.0, 240.0, 100.0, 0.7});
     } else {
         block = kBlock;
         w.lanes = Dk <= 32 ? 1 : Dk <= 64 ? 2 : Dk <= 128 ? 4 : 8;
@@ -90,6 +91,8 @@ struct Pass {
     bool exact_state;              // the state in all 24 bits although none is asked for
     const float *state_in;
     float *state_out;
+    const fss_heads *dot_with = nullptr;      // see mma::Dots
+    float *dots = nullptr;
 };
 
 static Problem make_problem(const fss_linear_attention *p, const Pass &s, const Plan &w, void *scratch) {
@@ -153,9 +156,10 @@ static bool make_map(CUtensorMap *map, const fss_heads &x, int64_t B, int64_t T)
 }
 
 template <typename T, typename TO, int KD, int kLoad, int kInput, int kState, int kKeys, bool kBoxed>
-static int run_chunked(const Problem &x, const Plan &w, const Pass &s, const fss_heads *o, const mma::Maps &maps, int flags, int32_t *status, cudaStream_t stream) {
+static int run_chunked(const Problem &x, const Plan &w, const Pass &s, const fss_heads *o, const mma::Maps &maps, int vec, int32_t *status, cudaStream_t stream) {
     const auto q = make_heads<const T>(&s.q, x.H), k = make_heads<const T>(&s.k, x.H), v = make_heads<const T>(&s.v, x.H);
     const auto out = make_heads<TO>(o, x.H);
+    const mma::Dots<T> dots{make_heads<const T>(s.dots ? s.dot_with : &s.q, x.H), s.dots};
     const int64_t blocks = x.B * x.H * w.nseg * w.v_tiles;
     if (blocks > INT32_MAX) return FSS_E_SHAPE;
     constexpr int few = mma::Plan<KD, kInput, kState, kKeys, false, false>::kShared, all = mma::Plan<KD, kInput, kState, kKeys, true, kBoxed>::kShared;
@@ -164,14 +168,14 @@ static int run_chunked(const Problem &x, const Plan &w, const Pass &s, const fss
     FSS_CUDA(cudaFuncSetAttribute(outputs, cudaFuncAttributeMaxDynamicSharedMemorySize, all), "shared memory of a chunked pass");
     if (w.nseg > 1) {
         FSS_CUDA(cudaFuncSetAttribute(sums, cudaFuncAttributeMaxDynamicSharedMemorySize, few), "shared memory of a chunked pass");
-        sums<<<(unsigned)(blocks / w.nseg * (w.nseg - 1)), mma::kThreads, few, stream>>>(x, maps, q, k, v, out, w.v_tiles, flags, status);
+        sums<<<(unsigned)(blocks / w.nseg * (w.nseg - 1)), mma::kThreads, few, stream>>>(x, maps, q, k, v, out, dots, w.v_tiles, vec, status);
         if (x.folded)
             FSS_CUDA(launch_dependent(fold_segments, dim3((unsigned)(x.B * x.H * ceil_div((int64_t)x.Dk * x.Dv, 256))), dim3(256), 0, stream, x),
                      "fold of the segments");
-        FSS_CUDA(launch_dependent(outputs, dim3((unsigned)blocks), dim3(mma::kThreads), all, stream, x, maps, q, k, v, out, w.v_tiles, flags, status),
+        FSS_CUDA(launch_dependent(outputs, dim3((unsigned)blocks), dim3(mma::kThreads), all, stream, x, maps, q, k, v, out, dots, w.v_tiles, vec, status),
                  "linear attention launch");
     } else {
-        outputs<<<(unsigned)blocks, mma::kThreads, all, stream>>>(x, maps, q, k, v, out, w.v_tiles, flags, status);
+        outputs<<<(unsigned)blocks, mma::kThreads, all, stream>>>(x, maps, q, k, v, out, dots, w.v_tiles, vec, status);
     }
     return launch_check("linear attention launch");
 }
@@ -199,6 +203,7 @@ template <typename T, typename TO> static int run_pass(const fss_linear_attentio
                 return tma ? FSS_CHUNKED(mma::kTma, 1, 1, 2, false) : FSS_CHUNKED(mma::kPlain, 1, 1, 2, false);
             } else {
                 // (where TMA cannot address one of the tensors, all go by ordinary accesses)
+                if (fine) return tma ? FSS_CHUNKED(mma::kTma, 1, 3, 3, false) : FSS_CHUNKED(mma::kPlain, 1, 3, 3, false);
                 const bool boxed = tma && make_map(&maps.o, *o, x.B, x.T);
                 if (s.exact_state || x.state_out) return boxed ? FSS_CHUNKED(mma::kTma, 1, 1, 3, true) : FSS_CHUNKED(mma::kPlain, 1, 1, 3, false);
                 return boxed ? FSS_CHUNKED(mma::kTma, 1, 1, 2, true) : FSS_CHUNKED(mma::kPlain, 1, 1, 2, false);
@@ -223,8 +228,10 @@ static BackwardPlan plan_backward(const fss_linear_attention *p, bool decays) {
     const bool f32 = p->dtype == FSS_DTYPE_F32;
     const size_t a = make_plan(p->B, p->T, p->H, Dv, Dk, decays || f32).seg_bytes, b = make_plan(p->B, p->T, p->H, Dk, Dv, f32).seg_bytes;
     w.seg = a > b ? a : b;
-    w.dq_each = decays || p->q.heads < p->H;
-    w.dk_each = decays || p->k.heads < p->H;
+    // the chunked kernels make the decays' dot products themselves, of up to 128 channels and where no heads are shared
+    const bool beside = make_plan(p->B, p->T, p->H, Dv, Dk, true).matrix && Dk <= mma::kValues;
+    w.dq_each = (decays && !beside) || p->q.heads < p->H;
+    w.dk_each = (decays && !beside) || p->k.heads < p->H;
     w.dv_each = p->v.heads < p->H;
     const int64_t widest = (w.dq_each || w.dk_each) && (Dk > Dv || !w.dv_each) ? Dk : w.dv_each ? Dv : 0;
     w.each = align_up((size_t)(n * widest) * sizeof(float), 256);
@@ -237,7 +244,12 @@ static BackwardPlan plan_backward(const fss_linear_attention *p, bool decays) {
 template <typename T>
 static int run_gradient(const fss_linear_attention *p, const Pass &s, const fss_heads &x, const fss_heads *dx, bool by_state, float *each, float *dots,
                         void *scratch, int32_t *status, cudaStream_t stream) {
-    if (!by_state) return run_pass<T, T>(p, s, dx, false, scratch, status, stream);
+    if (!by_state) {
+        Pass with = s;
+        with.dot_with = &x;
+        with.dots = dots;
+        return run_pass<T, T>(p, with, dx, dots != nullptr, scratch, status, stream);
+    }
     const int64_t D = s.v.dim;
     const fss_heads o{each, p->T * p->H * D, p->H * D, D, p->H, D};
     const int rc = run_pass<T, float>(p, s, &o, dots != nullptr, scratch, status, stream);

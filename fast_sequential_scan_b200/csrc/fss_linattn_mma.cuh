@@ -59,6 +59,13 @@ template <int KD, int kInput, int kState, int kKeys, bool kOut, bool kBoxed> str
 
 struct Maps { CUtensorMap q, k, v, o; };
 
+// What a gradient's outputs are multiplied with, for the decays' gradients: sums[b, t, h] = o . x, in fp32 before o is rounded.
+// sums NULL: not wanted.  One value tile; x has a head for each state.
+template <typename T> struct Dots {
+    Heads<const T> x;
+    float *sums;
+};
+
 // What a chunk's decays come to, by row.
 struct __align__(16) Decays {
     float enter[kChunk];      // e^{G_i} times the outputs' scale
@@ -215,13 +222,14 @@ template <typename T, int kPadded> struct Rows {
 
 template <typename T, typename TO, int KD, int kLoad, int kInput, int kState, int kKeys, bool kOut, bool kBoxed>
 __global__ void __launch_bounds__(kThreads, kOut && kState > 1 ? 1 : kInput > 1 ? 1 : 2)
-    chunked(Problem p, const __grid_constant__ Maps maps, Heads<const T> q, Heads<const T> k, Heads<const T> v, Heads<TO> o, int v_tiles, int flags,
-            int32_t *status) {
+    chunked(Problem p, const __grid_constant__ Maps maps, Heads<const T> q, Heads<const T> k, Heads<const T> v, Heads<TO> o, Dots<T> dots, int v_tiles,
+            int flags, int32_t *status) {
     using L = Plan<KD, kInput, kState, kKeys, kOut, kBoxed>;
     extern __shared__ char raw[];
     __shared__ Decays decays[2];
     __shared__ __align__(8) uint64_t barriers[3];
     __shared__ uint32_t tmem_slot;
+    __shared__ float dot_parts[kState == 3 && kOut ? kThreads / 32 : 1][32];
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, half = warp / 4;
     const uint32_t base = (umma::shared_address(raw) + 1023u) & ~1023u;
     const uint32_t loaded = umma::shared_address(&barriers[0]), scored = umma::shared_address(&barriers[1]), added = umma::shared_address(&barriers[2]);
@@ -241,6 +249,7 @@ __global__ void __launch_bounds__(kThreads, kOut && kState > 1 ? 1 : kInput > 1 
     const T *k_rows = k.row(b, 0, h), *q_rows = kOut ? q.row(b, 0, h) : nullptr, *v_rows = v.row(b, 0, h) + vt * kValues;
     const int k_head = (int)(h / k.group), q_head = kOut ? (int)(h / q.group) : 0, v_head = (int)(h / v.group);
     TO *out = kOut ? o.row(b, 0, h) + vt * kValues : nullptr;
+    const T *dot_rows = kState == 3 && kOut && dots.sums ? dots.x.row(b, 0, h) + min((warp % 4) * 32 + lane, Dv - 1) : nullptr;
     bool gave_up = false;
 
     if (warp == 0) umma::tmem_alloc<L::kColumns>(umma::shared_address(&tmem_slot));
@@ -530,6 +539,16 @@ __global__ void __launch_bounds__(kThreads, kOut && kState > 1 ? 1 : kInput > 1 
         }
         // fp32 rows travel while the products are made and the state and the outputs are seen to: there are registers for them
         // where a multiprocessor has one CTA
+        // rows of this half that are there
+        const int from = p.reverse ? max(kChunk - there - half * 32, 0) : 0, until = p.reverse ? 32 : min(there - half * 32, 32);
+        T with[kState == 3 && kOut ? 32 : 1] = {};      // this lane's channel of what the outputs are multiplied with
+        if constexpr (kState == 3 && kOut)
+            if (dots.sums && from < until) {
+                // (addresses that are there for every lane and token, so that the loads need no conditions and travel together)
+                const T *row = dot_rows + (int64_t)(t0 + half * 32) * dots.x.st;
+#pragma unroll
+                for (int i = 0; i < 32; ++i) with[i] = row[min(max(i, from), until - 1) * dots.x.st];
+            }
         constexpr bool kEarly = kLoad == kPlain && kInput > 1;
         const bool more_to_come = s0 + kChunk < stop;
         if (kEarly && more_to_come) fetch_keys(s0 + kChunk);
@@ -583,8 +602,7 @@ __global__ void __launch_bounds__(kThreads, kOut && kState > 1 ? 1 : kInput > 1 
         } else if (kOut && !kBoxed && !idle) {
             // lane = value channel, this half's 32 tokens
             TO *to = out + (int64_t)(t0 + half * 32) * o.st + dv;
-            // rows of this half that are there
-            const int from = p.reverse ? kChunk - there - half * 32 : 0, until = p.reverse ? 32 : there - half * 32;
+            float product[kState == 3 ? 32 : 1];
 #pragma unroll
             for (int i0 = 0; i0 < 32; i0 += 16) {
                 uint32_t r1[16], r2[16];
@@ -599,16 +617,44 @@ __global__ void __launch_bounds__(kThreads, kOut && kState > 1 ? 1 : kInput > 1 
                                         fmaf(f.z, __uint_as_float(r1[e + 2]), __uint_as_float(r2[e + 2])),
                                         fmaf(f.w, __uint_as_float(r1[e + 3]), __uint_as_float(r2[e + 3]))};
 #pragma unroll
-                    for (int u = 0; u < 4; ++u, to += o.st)
-                        if (dv < Dv && (full || (i0 + e + u >= from && i0 + e + u < until))) *to = (TO)x[u];
+                    for (int u = 0; u < 4; ++u, to += o.st) {
+                        const bool here = dv < Dv && (full || (i0 + e + u >= from && i0 + e + u < until));
+                        if (here) *to = (TO)x[u];
+                        if constexpr (kState == 3) {
+                            const float y = x[u] * (float)with[i0 + e + u];
+                            product[i0 + e + u] = here ? y : 0.f;
+                        }
+                    }
                 }
             }
+            if constexpr (kState == 3)
+                if (dots.sums) {
+                    // the lanes share the 32 tokens out: each step halves the tokens that a lane still adds up, until it has its own
+#pragma unroll
+                    for (int w = 16; w; w >>= 1) {
+                        const bool up = lane & w;
+#pragma unroll
+                        for (int i = 0; i < w; ++i) {
+                            const float mine = up ? product[i + w] : product[i], other = up ? product[i] : product[i + w];
+                            product[i] = mine + __shfl_xor_sync(0xffffffffu, other, w);
+                        }
+                    }
+                    dot_parts[warp][lane] = product[0];
+                }
         }
         if (kEarly && more_to_come) put_values();
         umma::fence_async_shared();
         umma::before_sync();
         __syncthreads();
         umma::after_sync();
+        if constexpr (kState == 3 && kOut)
+            if (dots.sums && threadIdx.x < kChunk) {
+                // warps 4 n .. 4 n + 3 had the value channels of half n's tokens; those of padding channels left nothing
+                const int row = threadIdx.x;
+                float sum = 0.f;
+                for (int w = 0; w < (Dv + 31) / 32; ++w) sum += dot_parts[row / 32 * 4 + w][row % 32];
+                if (full || (p.reverse ? row >= kChunk - there : row < there)) dots.sums[(b * p.T + t0 + row) * p.H + h] = sum;
+            }
         if (kBoxed && full) {
             if (threadIdx.x == 64) {
                 for (int c = 0; c < v_panels; ++c) umma::tma_store(&maps.o, base + L::kY + c * kPanel, vt * kValues + c * 64, (int)h, t0, (int)b);

@@ -21,6 +21,14 @@ namespace norm {
 constexpr float kLargest = 448.f;      // of e4m3
 constexpr float kLeast = 1e-30f;       // rows with no larger value than this are held as zeros times their scale
 
+// Row number to sequence and token.  (A division of 64 bits is as much work as the rest of a narrow row; tensors whose rows
+// are evenly spaced come as one long sequence.)
+struct Place { int64_t b, t; };
+__device__ __forceinline__ Place place(int64_t row, int64_t T) {
+    if (row < T) return {0, row};
+    return {row / T, row % T};
+}
+
 enum Quant { kNone = 0, kRow = 1, kGroup = 2 };
 
 template <typename T> struct Params {
@@ -103,13 +111,13 @@ template <int V> __device__ __forceinline__ void store_held(__nv_fp8_e4m3 *p, co
 struct Sum { static __device__ __forceinline__ float of(float a, float b) { return a + b; } };
 struct Most { static __device__ __forceinline__ float of(float a, float b) { return max_nan(a, b); } };
 
+// `shared`: 32 values for each use; a use and the one before it must not have the same.
 template <bool kBlockRow, typename Op> __device__ __forceinline__ float over_row(float x, float *shared) {
 #pragma unroll
     for (int w = 16; w; w >>= 1) x = Op::of(x, __shfl_xor_sync(0xffffffffu, x, w));
     if (!kBlockRow) return x;
     const int warps = blockDim.x / 32;
     if (warps == 1) return x;
-    __syncthreads();      // (the values of the sum before are read)
     if (threadIdx.x % 32 == 0) shared[threadIdx.x / 32] = x;
     __syncthreads();
     x = shared[0];
@@ -122,11 +130,11 @@ template <bool kBlockRow, typename Op> __device__ __forceinline__ float over_row
 template <typename T, int N, bool kBlockRow, int kQuant>
 __global__ void __launch_bounds__(kBlockRow ? 1024 : 256) forward(Params<T> p, bool wide) {
     constexpr int V = VecWidth<T>::value;
-    __shared__ float shared[32];
+    __shared__ float shared[2][32];
     const int threads = kBlockRow ? blockDim.x : 32, me = kBlockRow ? threadIdx.x : threadIdx.x % 32;
     const int64_t row = kBlockRow ? blockIdx.x : (int64_t)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
     if (row >= p.B * p.T_) return;      // (whole warps)
-    const int64_t b = row / p.T_, t = row % p.T_;
+    const auto [b, t] = place(row, p.T_);
     const int n = (int)(p.D / V);
     const T *x = p.x.row(b, t), *res = p.residual.ptr ? p.residual.row(b, t) : nullptr;
     typename Frag<T, V>::Raw raw[N], more[N];
@@ -155,7 +163,7 @@ __global__ void __launch_bounds__(kBlockRow ? 1024 : 256) forward(Params<T> p, b
             for (int i = 0; i < V; ++i) sum = fmaf(f[j][i], f[j][i], sum);
         }
     }
-    sum = over_row<kBlockRow, Sum>(sum, shared);
+    sum = over_row<kBlockRow, Sum>(sum, shared[0]);
     const float r = rsqrtf(sum / (float)p.D + p.eps);
     if (p.rstd && me == 0) p.rstd[row] = r;
     float most = 0.f;
@@ -174,7 +182,7 @@ __global__ void __launch_bounds__(kBlockRow ? 1024 : 256) forward(Params<T> p, b
         }
     }
     if (kQuant == kRow) {
-        most = over_row<kBlockRow, Most>(most, shared);
+        most = over_row<kBlockRow, Most>(most, shared[1]);
         if (me == 0) p.scales[row] = most / kLargest;
         const float inverse = kLargest / max_nan(most, kLeast);
 #pragma unroll
@@ -206,8 +214,10 @@ __global__ void __launch_bounds__(kBlockRow ? 1024 : 256) forward(Params<T> p, b
 // ------------------------------------------------------------------ forward, any width, alignment and type
 // A CTA for each row, one channel at a time; the row is read again for the output.
 template <typename T, int kQuant> __global__ void __launch_bounds__(256) forward_any(Params<T> p, bool wide) {
-    __shared__ float shared[32];
-    const int64_t row = blockIdx.x, b = row / p.T_, t = row % p.T_;
+    __shared__ float shared[2][32];
+    const int64_t row = blockIdx.x;
+    const auto [b0, t0] = place(row, p.T_);
+    const int64_t b = b0, t = t0;      // (a lambda takes no structured binding)
     const T *x = p.x.row(b, t), *res = p.residual.ptr ? p.residual.row(b, t) : nullptr;
     const T *kept = res ? p.sum.row(b, t) : x;      // (a thread reads back what it wrote itself)
     const auto value = [&](int64_t d) { return (float)kept[d]; };
@@ -222,7 +232,7 @@ template <typename T, int kQuant> __global__ void __launch_bounds__(256) forward
         const float f = value(d);
         sum = fmaf(f, f, sum);
     }
-    sum = over_row<true, Sum>(sum, shared);
+    sum = over_row<true, Sum>(sum, shared[0]);
     const float r = rsqrtf(sum / (float)p.D + p.eps);
     if (p.rstd && threadIdx.x == 0) p.rstd[row] = r;
     if (kQuant == kNone) {
@@ -234,7 +244,7 @@ template <typename T, int kQuant> __global__ void __launch_bounds__(256) forward
     for (int64_t g = 0; g < groups; ++g) {
         float most = 0.f;
         for (int64_t d = g * run + threadIdx.x; d < (g + 1) * run; d += blockDim.x) most = max_nan(most, fabsf(value(d) * r * weight(d)));
-        most = over_row<true, Most>(most, shared);
+        most = over_row<true, Most>(most, shared[(g + 1) % 2]);
         if (threadIdx.x == 0) p.scales[row * groups + g] = most / kLargest;
         const float inverse = kLargest / max_nan(most, kLeast);
         for (int64_t d = g * run + threadIdx.x; d < (g + 1) * run; d += blockDim.x) {
@@ -257,67 +267,103 @@ template <typename T> struct BackwardParams {
     float *parts;                   // NULL: the weight's gradient is not wanted
 };
 
+// kRows rows of a walker travel together, and share a barrier.
 template <typename T, int N, bool kBlockRow>
 __global__ void __launch_bounds__(kBlockRow ? 1024 : 256) backward(BackwardParams<T> p, bool wide) {
-    constexpr int V = VecWidth<T>::value;
-    __shared__ float shared[32];
-    const int threads = kBlockRow ? blockDim.x : 32, me = kBlockRow ? threadIdx.x : threadIdx.x % 32;
+    constexpr int V = VecWidth<T>::value, kRows = N == 1 ? 2 : 1;
+    __shared__ float shared[2][kRows][32];
+    const int threads = kBlockRow ? blockDim.x : 32, me = kBlockRow ? threadIdx.x : threadIdx.x % 32, warps = blockDim.x / 32;
     const int64_t walkers = kBlockRow ? gridDim.x : (int64_t)gridDim.x * (blockDim.x / 32);
     const int64_t walker = kBlockRow ? blockIdx.x : (int64_t)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
+    const int64_t rows = p.B * p.T_;
     const int n = (int)(p.D / V);
     float dw[N][V];
 #pragma unroll
     for (int j = 0; j < N; ++j)
 #pragma unroll
         for (int i = 0; i < V; ++i) dw[j][i] = 0.f;
-    for (int64_t row = walker; row < p.B * p.T_; row += walkers) {
-        const int64_t b = row / p.T_, t = row % p.T_;
-        typename Frag<T, V>::Raw rs[N], rg[N], ra[N];
-        const float r = p.rstd[row];
+    int turn = 0;
+    for (int64_t row0 = walker; row0 < rows; row0 += kRows * walkers) {
+        typename Frag<T, V>::Raw rs[kRows][N], rg[kRows][N], ra[kRows][N];
+        float r[kRows], dot[kRows];
 #pragma unroll
-        for (int j = 0; j < N; ++j) {
-            const int at = me + j * threads;
-            if (at < n) {
-                rs[j] = Frag<T, V>::load_raw(p.s.row(b, t) + (int64_t)at * V);
-                rg[j] = Frag<T, V>::load_raw(p.dy.row(b, t) + (int64_t)at * V);
-                if (p.dsum.ptr) ra[j] = Frag<T, V>::load_raw(p.dsum.row(b, t) + (int64_t)at * V);
-            }
-        }
-        float dot = 0.f;
+        for (int k = 0; k < kRows; ++k) {
+            const int64_t row = row0 + k * walkers;
+            r[k] = dot[k] = 0.f;
+            if (row >= rows) continue;
+            const auto [b, t] = place(row, p.T_);
+            r[k] = p.rstd[row];
 #pragma unroll
-        for (int j = 0; j < N; ++j) {
-            const int at = me + j * threads;
-            if (at < n) {
-                float s[V], g[V], w[V];
-                Frag<T, V>::unpack(rs[j], s);
-                Frag<T, V>::unpack(rg[j], g);
-                load_weight<V>(p.weight, wide, (int64_t)at * V, w);
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    dw[j][i] = fmaf(g[i], s[i] * r, dw[j][i]);
-                    dot = fmaf(g[i] * w[i], s[i], dot);
+            for (int j = 0; j < N; ++j) {
+                const int at = me + j * threads;
+                if (at < n) {
+                    rs[k][j] = Frag<T, V>::load_raw(p.s.row(b, t) + (int64_t)at * V);
+                    rg[k][j] = Frag<T, V>::load_raw(p.dy.row(b, t) + (int64_t)at * V);
+                    if (p.dsum.ptr) ra[k][j] = Frag<T, V>::load_raw(p.dsum.row(b, t) + (int64_t)at * V);
                 }
             }
         }
-        dot = over_row<kBlockRow, Sum>(dot, shared);
-        const float c = dot / (float)p.D * r * r * r;
 #pragma unroll
         for (int j = 0; j < N; ++j) {
             const int at = me + j * threads;
             if (at < n) {
-                float s[V], g[V], w[V];
-                Frag<T, V>::unpack(rs[j], s);
-                Frag<T, V>::unpack(rg[j], g);
+                float w[V];
                 load_weight<V>(p.weight, wide, (int64_t)at * V, w);
 #pragma unroll
-                for (int i = 0; i < V; ++i) g[i] = fmaf(g[i] * w[i], r, -s[i] * c);
-                if (p.dsum.ptr) {
-                    float a[V];
-                    Frag<T, V>::unpack(ra[j], a);
+                for (int k = 0; k < kRows; ++k) {
+                    if (row0 + k * walkers >= rows) continue;
+                    float s[V], g[V];
+                    Frag<T, V>::unpack(rs[k][j], s);
+                    Frag<T, V>::unpack(rg[k][j], g);
 #pragma unroll
-                    for (int i = 0; i < V; ++i) g[i] += a[i];
+                    for (int i = 0; i < V; ++i) {
+                        dw[j][i] = fmaf(g[i], s[i] * r[k], dw[j][i]);
+                        dot[k] = fmaf(g[i] * w[i], s[i], dot[k]);
+                    }
                 }
-                Frag<T, V>::store(p.dx.row(b, t) + (int64_t)at * V, g);
+            }
+        }
+#pragma unroll
+        for (int w = 16; w; w >>= 1)
+#pragma unroll
+            for (int k = 0; k < kRows; ++k) dot[k] += __shfl_xor_sync(0xffffffffu, dot[k], w);
+        if (kBlockRow && warps > 1) {
+#pragma unroll
+            for (int k = 0; k < kRows; ++k)
+                if (threadIdx.x % 32 == 0) shared[turn][k][threadIdx.x / 32] = dot[k];
+            __syncthreads();      // (the one of the rows before this guards the other half)
+#pragma unroll
+            for (int k = 0; k < kRows; ++k) {
+                dot[k] = shared[turn][k][0];
+                for (int w = 1; w < warps; ++w) dot[k] += shared[turn][k][w];
+            }
+            turn ^= 1;
+        }
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int at = me + j * threads;
+            if (at < n) {
+                float w[V];
+                load_weight<V>(p.weight, wide, (int64_t)at * V, w);
+#pragma unroll
+                for (int k = 0; k < kRows; ++k) {
+                    const int64_t row = row0 + k * walkers;
+                    if (row >= rows) continue;
+                    const float c = dot[k] / (float)p.D * r[k] * r[k] * r[k];
+                    float s[V], g[V];
+                    Frag<T, V>::unpack(rs[k][j], s);
+                    Frag<T, V>::unpack(rg[k][j], g);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) g[i] = fmaf(g[i] * w[i], r[k], -s[i] * c);
+                    if (p.dsum.ptr) {
+                        float a[V];
+                        Frag<T, V>::unpack(ra[k][j], a);
+#pragma unroll
+                        for (int i = 0; i < V; ++i) g[i] += a[i];
+                    }
+                    const Place to = place(row, p.T_);
+                    Frag<T, V>::store(p.dx.row(to.b, to.t) + (int64_t)at * V, g);
+                }
             }
         }
     }
@@ -333,7 +379,7 @@ __global__ void __launch_bounds__(kBlockRow ? 1024 : 256) backward(BackwardParam
 
 // Any width and alignment: CTA c takes the rows c, c + parts, ...; its sums go to its own row of `parts` in memory.
 template <typename T> __global__ void __launch_bounds__(256) backward_any(BackwardParams<T> p, bool wide) {
-    __shared__ float shared[32];
+    __shared__ float shared[2][32];
     const auto weight = [&](int64_t d) {
         float w[1];
         load_weight<1>(p.weight, wide, d, w);
@@ -342,8 +388,9 @@ template <typename T> __global__ void __launch_bounds__(256) backward_any(Backwa
     float *part = p.parts ? p.parts + blockIdx.x * p.D : nullptr;
     if (part)
         for (int64_t d = threadIdx.x; d < p.D; d += blockDim.x) part[d] = 0.f;      // (each thread only ever touches its own channels)
+    int turn = 0;
     for (int64_t row = blockIdx.x; row < p.B * p.T_; row += gridDim.x) {
-        const int64_t b = row / p.T_, t = row % p.T_;
+        const auto [b, t] = place(row, p.T_);
         const T *s = p.s.row(b, t), *dy = p.dy.row(b, t), *dsum = p.dsum.ptr ? p.dsum.row(b, t) : nullptr;
         const float r = p.rstd[row];
         float dot = 0.f;
@@ -351,7 +398,8 @@ template <typename T> __global__ void __launch_bounds__(256) backward_any(Backwa
             dot = fmaf((float)dy[d] * weight(d), (float)s[d], dot);
             if (part) part[d] = fmaf((float)dy[d], (float)s[d] * r, part[d]);
         }
-        dot = over_row<true, Sum>(dot, shared);
+        dot = over_row<true, Sum>(dot, shared[turn]);
+        turn ^= 1;
         const float c = dot / (float)p.D * r * r * r;
         for (int64_t d = threadIdx.x; d < p.D; d += blockDim.x)
             p.dx.row(b, t)[d] = (T)(fmaf((float)dy[d] * weight(d), r, -(float)s[d] * c) + (dsum ? (float)dsum[d] : 0.f));

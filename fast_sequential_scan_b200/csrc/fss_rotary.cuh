@@ -16,7 +16,7 @@
 namespace fss {
 namespace rotary {
 
-constexpr int kThreads = 256, kMaxPairs = 512;
+constexpr int kThreads = 256, kMaxPairs = 512, kMaxTokens = 64, kBatch = 4;
 
 template <typename T> struct Side {      // queries or keys: [B, T, heads, D]
     const T *in;
@@ -37,9 +37,14 @@ template <typename T> struct Params {
     int splits;                          // CTAs that share a token group's heads
 };
 
-// V: channels of an access.  kInterleaved: neighbouring channels make a pair, else channels j and j + R / 2.
+// V: channels of an access; 1 takes any layout.  kInterleaved: neighbouring channels make a pair, else channels j and j + R / 2.
+//
+// A thread has the same place in a head for all its items, and walks the (token, head) pairs of its CTA, kBatch of them at a
+// time in flight: no divisions, and neighbouring threads on neighbouring channels.
 template <typename T, int V, bool kInterleaved, bool kInverse> __global__ void __launch_bounds__(kThreads) rotate(Params<T> p) {
+    constexpr int kOwn = kInterleaved && V == 1 ? 2 : V;      // channels of an item's access (a pair, one by one, in the narrow interleaved form)
     extern __shared__ float2 turned[];      // [tokens][R / 2]: cos, sin
+    __shared__ int64_t from[kMaxTokens][2];      // where the tokens' heads begin
     const int pairs = p.R / 2;
     const int64_t all = p.B * p.T_, first = (int64_t)(blockIdx.x / p.splits) * p.tokens;
     const int split = blockIdx.x % p.splits;
@@ -53,84 +58,74 @@ template <typename T, int V, bool kInterleaved, bool kInverse> __global__ void _
         sincospif((float)(int32_t)(phase >> 32) * 0x1p-31f, &s, &c);
         turned[i] = make_float2(c * p.magnitude, (kInverse ? -s : s) * p.magnitude);
     }
-    __syncthreads();
-    // items: fragments of the turned channels (two for "half"), then of the channels that pass through
-    const int per_turn = kInterleaved ? p.R / V : pairs / V, rest = (p.D - p.R) / V, per_head = per_turn + rest;
-    const int heads = p.side[0].heads + p.side[1].heads;
-    const int per_token = heads * per_head, items = tokens * per_token;
-    for (int i = split * kThreads + threadIdx.x; i < items; i += p.splits * kThreads) {
-        const int tok = i / per_token, j = i % per_token % per_head;
-        int h = i % per_token / per_head;
-        const Side<T> &x = p.side[h >= p.side[0].heads];
-        if (h >= p.side[0].heads) h -= p.side[0].heads;
-        const int64_t at = first + tok;
-        const T *in = x.in + at / p.T_ * x.sb + at % p.T_ * x.st + (int64_t)h * x.sh;
-        T *out = x.out + (at * x.heads + h) * p.D;
-        float a[V], b[V];
-        if (j >= per_turn) {
-            const int d = p.R + (j - per_turn) * V;
-            Frag<T, V>::load(in + d, a);
-            Frag<T, V>::store(out + d, a);
-        } else if (kInterleaved) {
-            const float2 *cs = turned + tok * pairs + j * (V / 2);
-            Frag<T, V>::load(in + j * V, a);
-#pragma unroll
-            for (int e = 0; e < V; e += 2) {
-                const float2 z = cs[e / 2];
-                b[e] = a[e] * z.x - a[(e + 1) % V] * z.y;
-                b[(e + 1) % V] = a[e] * z.y + a[(e + 1) % V] * z.x;
-            }
-            Frag<T, V>::store(out + j * V, b);
-        } else {
-            const float2 *cs = turned + tok * pairs + j * V;
-            Frag<T, V>::load(in + j * V, a);
-            Frag<T, V>::load(in + pairs + j * V, b);
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-                const float2 z = cs[e];
-                const float x0 = a[e] * z.x - b[e] * z.y;
-                b[e] = a[e] * z.y + b[e] * z.x;
-                a[e] = x0;
-            }
-            Frag<T, V>::store(out + j * V, a);
-            Frag<T, V>::store(out + pairs + j * V, b);
-        }
-    }
-}
-
-// Interleaved pairs of single channels (odd strides): the pair itself is the item.
-template <typename T, bool kInverse> __global__ void __launch_bounds__(kThreads) rotate_pairs(Params<T> p) {
-    extern __shared__ float2 turned[];
-    const int pairs = p.R / 2;
-    const int64_t all = p.B * p.T_, first = (int64_t)(blockIdx.x / p.splits) * p.tokens;
-    const int split = blockIdx.x % p.splits;
-    const int tokens = (int)min((int64_t)p.tokens, all - first);
-    for (int i = threadIdx.x; i < tokens * pairs; i += kThreads) {
-        const int64_t at = first + i / pairs;
-        const int64_t position = p.positions[at / p.T_ * p.psb + at % p.T_ * p.pst];
-        const uint64_t phase = (uint64_t)position * (uint64_t)p.turns[i % pairs];
-        float s, c;
-        sincospif((float)(int32_t)(phase >> 32) * 0x1p-31f, &s, &c);
-        turned[i] = make_float2(c * p.magnitude, (kInverse ? -s : s) * p.magnitude);
+    for (int i = threadIdx.x; i < 2 * tokens; i += kThreads) {
+        const int64_t at = first + i / 2, b = at / p.T_, t = at % p.T_;
+        from[i / 2][i % 2] = b * p.side[i % 2].sb + t * p.side[i % 2].st;
     }
     __syncthreads();
-    const int rest = p.D - p.R, per_head = pairs + rest, heads = p.side[0].heads + p.side[1].heads;
-    const int per_token = heads * per_head, items = tokens * per_token;
-    for (int i = split * kThreads + threadIdx.x; i < items; i += p.splits * kThreads) {
-        const int tok = i / per_token, j = i % per_token % per_head;
-        int h = i % per_token / per_head;
-        const Side<T> &x = p.side[h >= p.side[0].heads];
-        if (h >= p.side[0].heads) h -= p.side[0].heads;
-        const int64_t at = first + tok;
-        const T *in = x.in + at / p.T_ * x.sb + at % p.T_ * x.st + (int64_t)h * x.sh;
-        T *out = x.out + (at * x.heads + h) * p.D;
-        if (j >= pairs) {
-            out[p.R + j - pairs] = in[p.R + j - pairs];
-        } else {
-            const float2 z = turned[tok * pairs + j];
-            const float a = (float)in[2 * j], b = (float)in[2 * j + 1];
-            out[2 * j] = (T)(a * z.x - b * z.y);
-            out[2 * j + 1] = (T)(a * z.y + b * z.x);
+    // places in a head: fragments of the turned channels (two for "half"), then of the channels that pass through
+    const int per_turn = kInterleaved ? p.R / kOwn : pairs / V, rest = (p.D - p.R) / V, per_head = per_turn + rest;
+    const int queries = p.side[0].heads, heads = queries + p.side[1].heads;
+    const int walkers = per_head < kThreads ? kThreads / per_head : 1;      // (a head of more places than threads: a thread has several)
+    for (int j = threadIdx.x % per_head; j < per_head; j += per_head < kThreads ? per_head : kThreads) {
+        const bool turns = j < per_turn;
+        const int d = turns ? j * kOwn : p.R + (j - per_turn) * V;
+        const int walker = threadIdx.x / per_head;
+        if (walker >= walkers) break;
+        int head = walker + split * walkers, token = 0;
+        const int step = walkers * p.splits;
+        const auto settle = [&] {
+            while (head >= heads) { head -= heads; ++token; }
+        };
+        settle();
+        while (token < tokens) {
+            typename Frag<T, V>::Raw a[kBatch], b[kBatch];
+            T *out[kBatch];
+            int of[kBatch];      // token, or -1
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+                of[i] = token < tokens ? token : -1;
+                if (token >= tokens) continue;
+                const int side = head >= queries, h = head - (side ? queries : 0);
+                const Side<T> &x = p.side[side];
+                const T *in = x.in + from[token][side] + (int64_t)h * x.sh + d;
+                out[i] = x.out + ((first + token) * x.heads + h) * p.D + d;
+                a[i] = Frag<T, V>::load_raw(in);
+                if (turns && !kInterleaved) b[i] = Frag<T, V>::load_raw(in + pairs);
+                if (turns && kInterleaved && V == 1) b[i] = Frag<T, V>::load_raw(in + 1);
+                head += step;
+                settle();
+            }
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+                if (of[i] < 0) continue;
+                float x[V], y[V];
+                Frag<T, V>::unpack(a[i], x);
+                if (!turns) {
+                    Frag<T, V>::store(out[i], x);
+                } else if (kInterleaved && V > 1) {
+                    const float2 *cs = turned + of[i] * pairs + j * (V / 2);
+#pragma unroll
+                    for (int e = 0; e < V; e += 2) {
+                        const float2 z = cs[e / 2];
+                        y[e] = x[e] * z.x - x[(e + 1) % V] * z.y;
+                        y[(e + 1) % V] = x[e] * z.y + x[(e + 1) % V] * z.x;
+                    }
+                    Frag<T, V>::store(out[i], y);
+                } else {
+                    const float2 *cs = turned + of[i] * pairs + j * V;
+                    Frag<T, V>::unpack(b[i], y);
+#pragma unroll
+                    for (int e = 0; e < V; ++e) {
+                        const float2 z = cs[e];
+                        const float turned_x = x[e] * z.x - y[e] * z.y;
+                        y[e] = x[e] * z.y + y[e] * z.x;
+                        x[e] = turned_x;
+                    }
+                    Frag<T, V>::store(out[i], x);
+                    Frag<T, V>::store(out[i] + (kInterleaved ? 1 : pairs), y);
+                }
+            }
         }
     }
 }
