@@ -42,9 +42,14 @@ template <int KD, int kInput, int kState, int kKeys, bool kOut, bool kBoxed> str
     static constexpr int kPanels = KD / 64;
     static constexpr int kKeyPiece = kPanels * kPanel, kValuePiece = 2 * kPanel;
     // Q first: its product reads 128 rows, of which the upper half lies behind its panels
+    // Two chunks' keys and values at a time where only the sums are made (there is room, and nothing else to wait for)
+    static constexpr int kStages = kOut || kInput > 1 ? 1 : 2;
     static constexpr int kQ = 0, kK = kQ + (kOut ? kInput * kKeyPiece : 0), kV = kK + (kKeys > kInput ? kKeys : kInput) * kKeyPiece, kP = kV + kInput * kValuePiece;
     static constexpr int kY = kP + (kOut ? kState * kPanel : 0);      // outputs on their way, one piece of bf16
-    static constexpr int kEnd = kY + (kBoxed ? kValuePiece : 0);
+    static constexpr int kSecond = kY + (kBoxed ? kValuePiece : 0);      // the second stage: keys' first piece, values
+    static constexpr int kEnd = kSecond + (kStages == 2 ? kKeyPiece + kValuePiece : 0);
+    static __device__ __forceinline__ int keys(int stage, int piece) { return kStages == 2 && stage && piece == 0 ? kSecond : kK + piece * kKeyPiece; }
+    static __device__ __forceinline__ int values(int stage) { return kStages == 2 && stage ? kSecond + kKeyPiece : kV; }
     static constexpr int kShared = kEnd + 1024;      // (the base is moved up to a multiple of 1,024)
     // tensor memory
     static constexpr int kO1 = 0, kScores = 64, kAdded = kOut ? 128 : 0;
@@ -97,7 +102,6 @@ __device__ __forceinline__ float factor(Log x) { return exp2f(x.part) * power_of
 
 // One warp's share of a chunk's decays: of visits s0 .. s0 + 63, two for each lane, whose logarithms were fetched ahead.
 // Returns the chunk's sum.  Every warp that takes part makes the sums; `part` 0 .. 2 says which factors it makes of them.
-constexpr int kDecayWarps = 3, kFirstDecayWarp = 5;
 __device__ __forceinline__ Log chunk_decays(Decays *d, const Problem &p, int part, int s0, int len, const float (&logs)[2], int lane) {
     const Log g0 = in_base_2(logs[0]), g1 = in_base_2(logs[1]);
     Log sum = g0 + g1;
@@ -227,12 +231,13 @@ __global__ void __launch_bounds__(kThreads, kOut && kState > 1 ? 1 : kInput > 1 
     using L = Plan<KD, kInput, kState, kKeys, kOut, kBoxed>;
     extern __shared__ char raw[];
     __shared__ Decays decays[2];
-    __shared__ __align__(8) uint64_t barriers[3];
+    __shared__ __align__(8) uint64_t barriers[4];
     __shared__ uint32_t tmem_slot;
     __shared__ float dot_parts[kState == 3 && kOut ? kThreads / 32 : 1][32];
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, half = warp / 4;
     const uint32_t base = (umma::shared_address(raw) + 1023u) & ~1023u;
-    const uint32_t loaded = umma::shared_address(&barriers[0]), scored = umma::shared_address(&barriers[1]), added = umma::shared_address(&barriers[2]);
+    const uint32_t scored = umma::shared_address(&barriers[0]), added = umma::shared_address(&barriers[1]);
+    const auto loaded = [&](int stage) { return umma::shared_address(&barriers[2 + stage]); };
     int64_t id = blockIdx.x;
     const int vt = id % v_tiles;
     id /= v_tiles;
@@ -254,16 +259,16 @@ __global__ void __launch_bounds__(kThreads, kOut && kState > 1 ? 1 : kInput > 1 
 
     if (warp == 0) umma::tmem_alloc<L::kColumns>(umma::shared_address(&tmem_slot));
     if (threadIdx.x == 32) {
-        umma::barrier_init(loaded, kOut ? 3 : 2);
+        for (int stage = 0; stage < L::kStages; ++stage) umma::barrier_init(loaded(stage), kOut ? 3 : 2);
         umma::barrier_init(scored, 1);
         umma::barrier_init(added, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     // channels that no load writes
     if (kLoad == kTma && v_panels == 1)
-        for (int i = threadIdx.x; i < kPanel / 16; i += kThreads) {
+        for (int i = threadIdx.x; i < L::kStages * kPanel / 16; i += kThreads) {
             const uint32_t zero[4] = {0, 0, 0, 0};
-            store_shared16(base + L::kV + kPanel + i * 16, zero);
+            store_shared16(base + L::values(i / (kPanel / 16)) + kPanel + i % (kPanel / 16) * 16, zero);
         }
 
     // scores above the diagonal: the half of them that no thread makes
@@ -323,17 +328,17 @@ __global__ void __launch_bounds__(kThreads, kOut && kState > 1 ? 1 : kInput > 1 
         if (kOut) queries.template put<kInput>(base + L::kQ, L::kKeyPiece);
     };
     const auto put_values = [&] { values.template put<kInput>(base + L::kV, L::kValuePiece); };
-    const auto load = [&](int s0) {
+    const auto load = [&](int s0, int stage) {
         const int t0 = first_token(s0);
         if (kLoad == kTma) {
             // (a warp for each tensor: issuing takes a thread some hundred cycles)
             const auto fetch = [&](const CUtensorMap *map, int to, int panels, int x, int head) {
-                umma::barrier_expect(loaded, (uint32_t)(panels * kPanel));
-                for (int c = 0; c < panels; ++c) umma::tma_load(base + to + c * kPanel, map, x + c * 64, head, (int)t0, (int)b, loaded);
+                umma::barrier_expect(loaded(stage), (uint32_t)(panels * kPanel));
+                for (int c = 0; c < panels; ++c) umma::tma_load(base + to + c * kPanel, map, x + c * 64, head, t0, (int)b, loaded(stage));
             };
-            if (threadIdx.x == 64) fetch(&maps.k, L::kK, L::kPanels, 0, k_head);
+            if (threadIdx.x == 64) fetch(&maps.k, L::keys(stage, 0), L::kPanels, 0, k_head);
             if (kOut && threadIdx.x == 96) fetch(&maps.q, L::kQ, L::kPanels, 0, q_head);
-            if (threadIdx.x == 128) fetch(&maps.v, L::kV, v_panels, vt * kValues, v_head);
+            if (threadIdx.x == 128) fetch(&maps.v, L::values(stage), v_panels, vt * kValues, v_head);
         } else {
             fetch_keys(s0);
             put_keys();
@@ -342,7 +347,9 @@ __global__ void __launch_bounds__(kThreads, kOut && kState > 1 ? 1 : kInput > 1 
         }
     };
 
-    const bool decayer = warp >= kFirstDecayWarp && warp < kFirstDecayWarp + kDecayWarps;
+    // (warps that make no scores and issue no products)
+    const bool decayer = warp == 3 || warp >= 6;
+    const int decay_part = warp == 3 ? 0 : warp - 5;
     double total = 0.0;      // of these warps: the logarithm of the decay of all chunks
     float logs[2];           // of the next chunk's decays
     const auto fetch_logs = [&](int s0) {
@@ -350,10 +357,11 @@ __global__ void __launch_bounds__(kThreads, kOut && kState > 1 ? 1 : kInput > 1 
         for (int i = 0; i < 2; ++i) logs[i] = s0 + 2 * lane + i < len ? p.log_decay(b, h, s0 + 2 * lane + i, len) : 0.f;
     };
     if (begin < stop) {
-        load(begin);
+        load(begin, 0);
+        if (kLoad == kTma && L::kStages == 2 && begin + kChunk < stop) load(begin + kChunk, 1);
         if (decayer) {
             fetch_logs(begin);
-            const Log x = chunk_decays(&decays[0], p, warp - kFirstDecayWarp, begin, len, logs, lane);
+            const Log x = chunk_decays(&decays[0], p, decay_part, begin, len, logs, lane);
             total += (double)x.whole + x.part;
         }
         if (kOut) write_state();
@@ -363,24 +371,28 @@ __global__ void __launch_bounds__(kThreads, kOut && kState > 1 ? 1 : kInput > 1 
     __syncthreads();
     umma::after_sync();
 
-    uint32_t parity = 0, lost = 2;      // lost: the phase whose copies did not come
+    uint32_t parity = 0, lost = 2;      // lost: the phase whose copies did not come, of lost_stage
+    int lost_stage = 0;
     for (int s0 = begin; s0 < stop; s0 += kChunk, parity ^= 1) {
         const Decays &d = decays[parity];
         const int there = min(kChunk, stop - s0);      // tokens of the chunk
         const int t0 = first_token(s0);
         const bool full = there == kChunk;
+        // with two stages the chunks take turns, and a stage's phase changes every second chunk
+        const int stage = kLoad == kTma && L::kStages == 2 ? (int)parity : 0;
+        const uint32_t load_parity = kLoad == kTma && L::kStages == 2 ? (uint32_t)((s0 - begin) / kChunk / 2 & 1) : parity;
         if (decayer && s0 + kChunk < stop) fetch_logs(s0 + kChunk);
         if (kLoad == kTma) {
             const bool before = gave_up;
-            umma::barrier_wait(loaded, parity, gave_up);
-            if (gave_up && !before) lost = parity;
+            umma::barrier_wait(loaded(stage), load_parity, gave_up);
+            if (gave_up && !before) { lost = load_parity; lost_stage = stage; }
             if (there < kChunk) {
                 // Rows behind the sequence hold anything.  Scores and keys of such rows are replaced by zeros below; values
                 // meet those zeros in a product, so they have to be numbers.
                 for (int i = threadIdx.x; i < v_panels * kChunk * 8; i += kThreads) {
                     const int row = i / 8 % kChunk;
                     const uint32_t zero[4] = {0, 0, 0, 0};
-                    if ((p.reverse ? kChunk - 1 - row : row) >= there) store_shared16(base + L::kV + i / (8 * kChunk) * kPanel + row * 128 + i % 8 * 16, zero);
+                    if ((p.reverse ? kChunk - 1 - row : row) >= there) store_shared16(base + L::values(stage) + i / (8 * kChunk) * kPanel + row * 128 + i % 8 * 16, zero);
                 }
             }
         }
@@ -414,13 +426,13 @@ __global__ void __launch_bounds__(kThreads, kOut && kState > 1 ? 1 : kInput > 1 
         // the keys themselves, once the scores are made
         constexpr int kUnits = kChunk * KD / 8 / kThreads;
         uint32_t first_piece[kUnits][4];
-        const uint32_t k_base = fresh(base) + L::kK;
+        const uint32_t k_base = fresh(base);
 #pragma unroll
         for (int i = 0; i < kUnits; ++i) {
             const int at = threadIdx.x + i * kThreads, row = at / (KD / 8), c = at % (KD / 8) * 8;
             uint32_t unit[kInput][4], w[kKeys][4];
 #pragma unroll
-            for (int m = 0; m < kInput; ++m) load_shared16(unit_address(k_base + m * L::kKeyPiece, row, c), unit[m]);
+            for (int m = 0; m < kInput; ++m) load_shared16(unit_address(k_base + L::keys(stage, m), row, c), unit[m]);
             const Two f = splat(d.leave[row]);
             const bool here = full || (p.reverse ? kChunk - 1 - row : row) < there;
             if (kInput > 1 && kOut && i == 0) umma::barrier_wait(scored, parity, gave_up);      // all pieces lie over the keys'
@@ -437,14 +449,14 @@ __global__ void __launch_bounds__(kThreads, kOut && kState > 1 ? 1 : kInput > 1 
                 first_piece[i][j] = z[0];
             }
 #pragma unroll
-            for (int m = kInput > 1 ? 0 : 1; m < kKeys; ++m) store_shared16(unit_address(k_base + m * L::kKeyPiece, row, c), w[m]);
+            for (int m = kInput > 1 ? 0 : 1; m < kKeys; ++m) store_shared16(unit_address(k_base + L::keys(stage, m), row, c), w[m]);
         }
         if (kInput == 1) {
             if (kOut) umma::barrier_wait(scored, parity, gave_up);
 #pragma unroll
             for (int i = 0; i < kUnits; ++i) {
                 const int at = threadIdx.x + i * kThreads, row = at / (KD / 8), c = at % (KD / 8) * 8;
-                store_shared16(unit_address(k_base, row, c), first_piece[i]);
+                store_shared16(unit_address(k_base + L::keys(stage, 0), row, c), first_piece[i]);
             }
         }
         umma::after_sync();
@@ -508,7 +520,7 @@ __global__ void __launch_bounds__(kThreads, kOut && kState > 1 ? 1 : kInput > 1 
         umma::after_sync();
         if (threadIdx.x == 64) {
             const uint32_t from = fresh(base);
-            const uint64_t values = umma::operand(from + L::kV, kPanel), scores = umma::operand(from + L::kP, 16), decayed = umma::operand(from + L::kK, kPanel);
+            const uint64_t values = umma::operand(from + L::values(stage), kPanel), scores = umma::operand(from + L::kP, 16);
             bool more = false;
             if (kOut) {
                 constexpr uint32_t what = umma::product(kValues, kChunk, true, false);
@@ -530,11 +542,11 @@ __global__ void __launch_bounds__(kThreads, kOut && kState > 1 ? 1 : kInput > 1 
 #pragma unroll
                     for (int s = 0; s < (a + c < 3 ? kChunk / 16 : 0); ++s, more = true)
                         umma::multiply(tmem + L::kAdded, values + ((a * L::kValuePiece + s * 2048) >> 4),
-                                       decayed + ((c * L::kKeyPiece + s * 2048) >> 4), what, more);
+                                       umma::operand(from + L::keys(stage, c) + s * 2048, kPanel), what, more);
             umma::tell_when_done(added);
         }
         if (decayer && s0 + kChunk < stop) {
-            const Log x = chunk_decays(&decays[parity ^ 1], p, warp - kFirstDecayWarp, s0 + kChunk, len, logs, lane);
+            const Log x = chunk_decays(&decays[parity ^ 1], p, decay_part, s0 + kChunk, len, logs, lane);
             if (!kOut) total += (double)x.whole + x.part;
         }
         // fp32 rows travel while the products are made and the state and the outputs are seen to: there are registers for them
@@ -557,8 +569,12 @@ __global__ void __launch_bounds__(kThreads, kOut && kState > 1 ? 1 : kInput > 1 
         if (kEarly && more_to_come) {
             put_keys();
             fetch_values(s0 + kChunk);
-        } else if (more_to_come && !(kLoad == kTma && gave_up)) {
-            load(s0 + kChunk);
+        } else if (kLoad == kTma) {
+            // into the stage that this chunk's products have let go of
+            const int next = s0 + L::kStages * kChunk;
+            if (next < stop && !gave_up) load(next, stage);
+        } else if (more_to_come) {
+            load(s0 + kChunk, 0);
         }
         const bool idle = warp % 4 * 32 >= Dv;      // this warp's value channels are padding
         const Two all = splat(d.all), rest = splat(d.rest);
@@ -675,7 +691,7 @@ __global__ void __launch_bounds__(kThreads, kOut && kState > 1 ? 1 : kInput > 1 
     if (gave_up) report_status(status, FSS_STATUS_TMA_TIMEOUT);
     if (lost < 2) {      // copies that are still on their way: another two seconds before the CTA leaves its shared memory
         bool again = false;
-        umma::barrier_wait(loaded, lost, again);
+        umma::barrier_wait(loaded(lost_stage), lost, again);
     }
     if (kOut) {
         const int z0 = max(begin, len);
@@ -685,7 +701,7 @@ __global__ void __launch_bounds__(kThreads, kOut && kState > 1 ? 1 : kInput > 1 
         float *to = kOut ? p.state_out + (b * p.H + h) * (int64_t)p.Dk * p.Dv : p.seg_state + ((b * p.H + h) * p.nseg + seg) * (int64_t)p.Dk * p.Dv;
         const int64_t sk = kOut ? p.sk : p.Dv, sv = kOut ? p.sv : 1;
         const float last = kOut && p.reverse && len > 0 ? expf(p.g[b * p.gsb + h * p.gsh]) : 1.f;
-        if (!kOut && vt == 0 && threadIdx.x == kFirstDecayWarp * 32) p.seg_decay[(b * p.H + h) * p.nseg + seg] = (float)exp2(total);
+        if (!kOut && vt == 0 && threadIdx.x == 96) p.seg_decay[(b * p.H + h) * p.nseg + seg] = (float)exp2(total);
 #pragma unroll
         for (int i = 0; i < kMine; ++i)
             if (dv < Dv && key0 + i < p.Dk) to[(key0 + i) * sk + (vt * kValues + dv) * sv] = state[i] * last;
