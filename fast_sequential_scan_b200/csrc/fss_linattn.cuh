@@ -82,13 +82,13 @@ struct Problem {
 // ------------------------------------------------------------------ the state that enters a segment
 // N key channels from `key0` on of the value channel `value` of the state that enters segment `seg`, for the kernels that
 // compute outputs; zeros where there is no such channel.  What the launch before this one wrote is read past the L1.
-// Every load has an address that is there and no condition, so that sixteen of them travel together.
+// Every load has an address that is there and no condition, so that 32 of them travel together.
 template <int N> __device__ __forceinline__ void entering_state(const Problem &p, int64_t b, int64_t h, int seg, int key0, int value, float (&state)[N]) {
     const int64_t bh = b * p.H + h, n = (int64_t)p.Dk * p.Dv;
     const int count = value < p.Dv ? p.Dk - key0 : 0;      // channels that are there
     const auto add = [&](const float *matrix, int64_t sk, int64_t sv, float decay) {
         const float *from = matrix + (int64_t)min(value, p.Dv - 1) * sv;
-        constexpr int kBatch = N < 16 ? N : 16;
+        constexpr int kBatch = N < 32 ? N : 32;
 #pragma unroll
         for (int i0 = 0; i0 < N; i0 += kBatch) {
             float x[kBatch];

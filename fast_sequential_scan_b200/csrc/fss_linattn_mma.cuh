@@ -284,10 +284,6 @@ __global__ void __launch_bounds__(kThreads, kOut && kState > 1 ? 1 : kInput > 1 
     float state[kMine];
 #pragma unroll
     for (int i = 0; i < kMine; ++i) state[i] = 0.f;
-    if (kOut) {
-        asm volatile("griddepcontrol.wait;" ::: "memory");      // the segments' sums are another launch's
-        entering_state(p, b, h, seg, key0, vt * kValues + dv, state);
-    }
     umma::fence_async_shared();
     umma::before_sync();
     __syncthreads();
@@ -364,7 +360,11 @@ __global__ void __launch_bounds__(kThreads, kOut && kState > 1 ? 1 : kInput > 1 
             const Log x = chunk_decays(&decays[0], p, decay_part, begin, len, logs, lane);
             total += (double)x.whole + x.part;
         }
-        if (kOut) write_state();
+    }
+    if (kOut) {
+        asm volatile("griddepcontrol.wait;" ::: "memory");      // the segments' sums are another launch's (the tokens are not)
+        entering_state(p, b, h, seg, key0, vt * kValues + dv, state);
+        if (begin < stop) write_state();
     }
     umma::fence_async_shared();
     umma::before_sync();
