@@ -205,7 +205,8 @@ template <typename T, typename TO> static int run_pass(const fss_linear_attentio
             } else {
                 // (where TMA cannot address one of the tensors, all go by ordinary accesses)
                 if (fine) return tma ? FSS_CHUNKED(mma::kTma, 1, 3, 3, false) : FSS_CHUNKED(mma::kPlain, 1, 3, 3, false);
-                const bool boxed = tma && make_map(&maps.o, *o, x.B, x.T);
+                // (the last chunk's rows are stored 16 bytes at a time)
+                const bool boxed = tma && x.Dv % 8 == 0 && make_map(&maps.o, *o, x.B, x.T);
                 if (s.exact_state || x.state_out) return boxed ? FSS_CHUNKED(mma::kTma, 1, 1, 3, true) : FSS_CHUNKED(mma::kPlain, 1, 1, 3, false);
                 return boxed ? FSS_CHUNKED(mma::kTma, 1, 1, 2, true) : FSS_CHUNKED(mma::kPlain, 1, 1, 2, false);
             }

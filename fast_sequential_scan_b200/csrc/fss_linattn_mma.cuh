@@ -379,8 +379,8 @@ __global__ void __launch_bounds__(kThreads, kOut && kState > 1 ? 1 : kInput > 1 
     __syncthreads();
     umma::after_sync();
 
-    uint32_t parity = 0, lost = 2;      // lost: the phase whose copies did not come, of lost_stage
-    int lost_stage = 0;
+    uint32_t parity = 0;
+    int lost = -1;      // the chunk whose copies did not come
     for (int s0 = begin; s0 < stop; s0 += kChunk, parity ^= 1) {
         const Decays &d = decays[parity];
         const int there = min(kChunk, stop - s0);      // tokens of the chunk
@@ -393,7 +393,7 @@ __global__ void __launch_bounds__(kThreads, kOut && kState > 1 ? 1 : kInput > 1 
         if (kLoad == kTma) {
             const bool before = gave_up;
             umma::barrier_wait(loaded(stage), load_parity, gave_up);
-            if (gave_up && !before) { lost = load_parity; lost_stage = stage; }
+            if (gave_up && !before) lost = (s0 - begin) / kChunk;
             if (there < kChunk) {
                 // Rows behind the sequence hold anything.  Scores and keys of such rows are replaced by zeros below; values
                 // meet those zeros in a product, so they have to be numbers.
@@ -697,9 +697,12 @@ __global__ void __launch_bounds__(kThreads, kOut && kState > 1 ? 1 : kInput > 1 
     }
     if (kBoxed && threadIdx.x == 64) umma::tma_wait_all();
     if (gave_up) report_status(status, FSS_STATUS_TMA_TIMEOUT);
-    if (lost < 2) {      // copies that are still on their way: another two seconds before the CTA leaves its shared memory
-        bool again = false;
-        umma::barrier_wait(loaded(lost_stage), lost, again);
+    if (kLoad == kTma && lost >= 0) {
+        // copies that are still on their way: another two seconds for each chunk of them before the CTA leaves its shared memory
+        for (int c = lost; c < lost + L::kStages && begin + c * kChunk < stop; ++c) {
+            bool again = false;
+            umma::barrier_wait(loaded(c % L::kStages), (uint32_t)(c / L::kStages & 1), again);
+        }
     }
     if (kOut) {
         const int z0 = max(begin, len);

@@ -307,6 +307,24 @@ def test_on_another_stream_and_in_a_graph():
     fss().check_status()
 
 
+@pytest.mark.parametrize("T", [70, 128])
+@pytest.mark.parametrize("V,pitch", [(52, 64), (64, 72), (40, 41)])
+def test_outputs_between_other_data(V, pitch, T):
+    """Rows of outputs with a gap behind each: nothing else is written (through the C entry; the Python functions make contiguous ones)."""
+    import ctypes
+    from fast_sequential_scan_b200 import _lib, attention_cuda, workspace
+    q, k, v, g, _, _ = make(2, T, 2, 64, V, BF16, decay="fixed", state=False)
+    v = torch.nn.functional.pad(v, (0, 64 - V))[..., :V]      # rows of 128 bytes
+    room = torch.full((2, T, 2, pitch), 7.0, device="cuda", dtype=BF16)
+    p = attention_cuda._problem(q, k, v, g, None, None, 0.125, 2, T)
+    out = _lib.Heads(room.data_ptr(), T * 2 * pitch, 2 * pitch, pitch, 2, V)
+    ctx = workspace.call_context(q.device, attention_cuda._scratch(p, 0, q.device))
+    _lib.check(_lib.lib().fss_linear_attention_forward(ctypes.byref(ctx), ctypes.byref(p), ctypes.byref(out), None), "forward")
+    fss().check_status()
+    assert relative(room[..., :V], oracle(q, k, v, g, 0.125)[0]) <= TOL[BF16]
+    assert (room[..., V:] == 7.0).all()
+
+
 # ------------------------------------------------------------------ single tokens
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("K,V", DIMS)
