@@ -115,15 +115,15 @@ static Problem make_problem(const fss_linear_attention *p, const Pass &s, const 
     return x;
 }
 
-template <typename T, typename TO, int L> static int run_recurrent(const Problem &x, const Plan &w, const Pass &s, const fss_heads *o, cudaStream_t stream) {
+template <typename T, typename TO, int L, int kLaneK> static int run_recurrent(const Problem &x, const Plan &w, const Pass &s, const fss_heads *o, cudaStream_t stream) {
     const auto q = make_heads<const T>(&s.q, x.H), k = make_heads<const T>(&s.k, x.H), v = make_heads<const T>(&s.v, x.H);
     const auto out = make_heads<TO>(o, x.H);
     const int vec = wide_rows(q, x.Dk) && wide_rows(k, x.Dk) && wide_rows(v, x.Dv);
     const int64_t blocks = x.B * x.H * w.nseg * w.v_tiles;
     if (blocks > INT32_MAX) return FSS_E_SHAPE;
-    const size_t smem = shared_bytes<L>(w.warps);
-    auto *sums = recurrent<T, TO, L, false>;
-    auto *outputs = recurrent<T, TO, L, true>;
+    const size_t smem = shared_bytes<L, kLaneK>(w.warps);
+    auto *sums = recurrent<T, TO, L, kLaneK, false>;
+    auto *outputs = recurrent<T, TO, L, kLaneK, true>;
     if (smem > 48 * 1024) {
         FSS_CUDA(cudaFuncSetAttribute(sums, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), "shared memory of a recurrent pass");
         FSS_CUDA(cudaFuncSetAttribute(outputs, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), "shared memory of a recurrent pass");
@@ -213,10 +213,12 @@ template <typename T, typename TO> static int run_pass(const fss_linear_attentio
         }
 #undef FSS_CHUNKED
     }
-    if (w.lanes == 1) return run_recurrent<T, TO, 1>(x, w, s, o, stream);
-    if (w.lanes == 2) return run_recurrent<T, TO, 2>(x, w, s, o, stream);
-    if (w.lanes == 4) return run_recurrent<T, TO, 4>(x, w, s, o, stream);
-    return run_recurrent<T, TO, 8>(x, w, s, o, stream);
+    if (w.lanes == 1) return run_recurrent<T, TO, 1, 32>(x, w, s, o, stream);
+    if (w.lanes == 2) return run_recurrent<T, TO, 2, 32>(x, w, s, o, stream);
+    if (w.lanes == 4) return run_recurrent<T, TO, 4, 32>(x, w, s, o, stream);
+    if (x.Dk <= 160) return run_recurrent<T, TO, 8, 20>(x, w, s, o, stream);
+    if (x.Dk <= 192) return run_recurrent<T, TO, 8, 24>(x, w, s, o, stream);
+    return run_recurrent<T, TO, 8, 32>(x, w, s, o, stream);
 }
 
 // ------------------------------------------------------------------ gradients

@@ -120,21 +120,23 @@ template <int N> __device__ __forceinline__ void entering_state(const Problem &p
 // Measured on B200: a training step of 2 x 65 tokens x 8 heads of 256 in fp32, 0.35 ms; one of 13 sequences of a token, 20 heads
 // of 64, 0.11 ms.  Up to 16 tokens the chunked kernels' fixed work is more than the tokens'.
 // Bound by the fp32 pipes: 4 Dk Dv operations a token against 2 (2 Dk + 2 Dv) or twice that many bytes.
-constexpr int kLaneK = 32, kLaneV = 4;
+constexpr int kLaneV = 4;
 constexpr int kBlock = 32;      // tokens staged in shared memory at a time (a warp's lanes take their decays)
-constexpr int kPitch = kLaneK + 4;                        // floats between the key channels of neighbouring lanes: other banks
 
-template <int L> struct Shape {
+// L lanes of kLaneK key channels each.  Fewer than 32 a lane for key dimensions from 129 to 192, because work goes by the
+// padded dimension.
+template <int L, int kLaneK> struct Shape {
     static constexpr int kColumns = 32 / L * kLaneV;      // value channels of a warp
+    static constexpr int kPitch = kLaneK % 8 == 4 ? kLaneK : kLaneK + 4;      // floats between neighbouring lanes' key channels: other banks
     static constexpr int kKeyRow = L * kPitch;
 };
 
-template <int L> inline size_t shared_bytes(int warps) {
-    return (size_t)kBlock * (2 * Shape<L>::kKeyRow + warps * Shape<L>::kColumns + 2) * sizeof(float);
+template <int L, int kLaneK> inline size_t shared_bytes(int warps) {
+    return (size_t)kBlock * (2 * Shape<L, kLaneK>::kKeyRow + warps * Shape<L, kLaneK>::kColumns + 2) * sizeof(float);
 }
 
 // rows of `n` channels (zeros up to `padded`) into shared memory as fp32; key rows are laid out in lane order
-template <typename T, bool kKeys>
+template <typename T, int kLaneK, int kPitch>      // kLaneK 0: values
 __device__ __forceinline__ void stage(float *to, int pitch, const Heads<const T> &x, const Problem &p, int64_t b, int64_t h, int64_t first, int rows,
                                       int64_t len, int offset, int n, int padded, float scale, bool vec) {
     constexpr int V = VecWidth<T>::value;
@@ -149,16 +151,17 @@ __device__ __forceinline__ void stage(float *to, int pitch, const Heads<const T>
 #pragma unroll
             for (int j = 0; j < V; ++j) f[j] = c + j < n ? (float)row[c + j] : 0.f;
         }
-        float *at = to + r * pitch + (kKeys ? c / kLaneK * kPitch + c % kLaneK : c);
 #pragma unroll
-        for (int j = 0; j < V; j += 4) *reinterpret_cast<float4 *>(at + j) = make_float4(f[j] * scale, f[j + 1] * scale, f[j + 2] * scale, f[j + 3] * scale);
+        for (int j = 0; j < V; j += 4)
+            *reinterpret_cast<float4 *>(to + r * pitch + (kLaneK ? (c + j) / (kLaneK ? kLaneK : 1) * kPitch + (c + j) % (kLaneK ? kLaneK : 1) : c + j)) = make_float4(f[j] * scale, f[j + 1] * scale, f[j + 2] * scale, f[j + 3] * scale);
     }
 }
 
 // kOut: outputs (and the last state, where there is one segment); else the segments' own sums.
-template <typename T, typename TO, int L, bool kOut>
+template <typename T, typename TO, int L, int kLaneK, bool kOut>
 __global__ void __launch_bounds__(128) recurrent(Problem p, Heads<const T> q, Heads<const T> k, Heads<const T> v, Heads<TO> o, int v_tiles, int vec) {
-    using S = Shape<L>;
+    using S = Shape<L, kLaneK>;
+    constexpr int kPitch = S::kPitch;
     extern __shared__ float4 smem4[];
     const int warps = blockDim.x / 32, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int tile = warps * S::kColumns;
@@ -189,9 +192,9 @@ __global__ void __launch_bounds__(128) recurrent(Problem p, Heads<const T> q, He
     for (int64_t s0 = begin; s0 < min(end, len); s0 += kBlock) {
         const int rows = (int)min((int64_t)kBlock, min(end, len) - s0);
         __syncthreads();
-        stage<T, true>(ks, S::kKeyRow, k, p, b, h, s0, rows, len, 0, p.Dk, L * kLaneK, 1.f, vec);
-        if (kOut) stage<T, true>(qs, S::kKeyRow, q, p, b, h, s0, rows, len, 0, p.Dk, L * kLaneK, 1.f, vec);
-        stage<T, false>(vs, tile, v, p, b, h, s0, rows, len, vt * tile, p.Dv - vt * tile, tile, p.in_scale, vec);
+        stage<T, kLaneK, kPitch>(ks, S::kKeyRow, k, p, b, h, s0, rows, len, 0, p.Dk, L * kLaneK, 1.f, vec);
+        if (kOut) stage<T, kLaneK, kPitch>(qs, S::kKeyRow, q, p, b, h, s0, rows, len, 0, p.Dk, L * kLaneK, 1.f, vec);
+        stage<T, 0, 0>(vs, tile, v, p, b, h, s0, rows, len, vt * tile, p.Dv - vt * tile, tile, p.in_scale, vec);
         if (threadIdx.x < rows) {      // (kBlock is a warp)
             const float e = p.log_decay(b, h, s0 + threadIdx.x, len);
             const double a = exp((double)e);

@@ -307,6 +307,13 @@ def test_on_another_stream_and_in_a_graph():
     fss().check_status()
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("K,V", [(129, 64), (144, 144), (160, 20), (161, 161), (192, 130), (193, 65)])
+def test_wide_keys(K, V, dtype):
+    check_forward(make(2, 77, 2, K, V, dtype, ragged=True, seed=K))
+    check_gradients(make(1, 50, 2, K, V, dtype, Hk=1, seed=V))
+
+
 @pytest.mark.parametrize("T", [70, 128])
 @pytest.mark.parametrize("V,pitch", [(52, 64), (64, 72), (40, 41)])
 def test_outputs_between_other_data(V, pitch, T):
